@@ -7,7 +7,7 @@
  * sizes, and return 0 on success or a non-zero wgb status; wgb_last_error()
  * returns the message of the last failure on the calling thread.
  *
- * Two groups of entry points:
+ * Three groups of entry points:
  *
  * 1. Drop-in replacements for the reference's PyTorch extension
  *    warpgbm.cuda.node_kernel (warpgbm/cuda/node_kernel.cpp:41-46).  Same
@@ -19,6 +19,10 @@
  *    one split search per level, an on-device partition, and no host
  *    synchronisation inside a tree.  It replaces the depth-first recursion
  *    of warpgbm/core.py:543-658 and 692-744.
+ *
+ * 3. Objectives on log-probabilities (no counterpart in the reference): label
+ *    log-probs of rows of logits, a preference loss over paired log ratios
+ *    and a clipped policy loss with a KL term, each with its gradient.
  */
 #ifndef WARPGBM_B200_H
 #define WARPGBM_B200_H
@@ -452,6 +456,109 @@ int wgb_predict_packed(const int8_t *bins, int64_t n, int64_t S,
 int wgb_predict_heap(const int8_t *bins, int64_t n, int64_t S,
                      const uint32_t *heap, int32_t T, int32_t K, int32_t D,
                      float lr, float *out, void *stream);
+
+/* ---------------------------------------------------------------------- */
+/* 3. objectives on log-probabilities                                       */
+/* ---------------------------------------------------------------------- */
+
+/* Common to this group.  logits: [rows][classes], dtype 0 float32, 1 bfloat16,
+ * 2 float16, unit stride along classes, `row_stride` elements between rows,
+ * aligned to its element.  z = logits / temperature.  labels: 4- or 8-byte
+ * integers (label_bytes); a negative label leaves its row out (zeros in every
+ * output), one that is not below `classes` gives NaN.  A logit of -inf is a
+ * masked place; a row that is all -inf has lse = logp = -inf, entropy 0 and a
+ * gradient of zeros.  Per-token arrays are float32; mask bytes: 0 leaves the
+ * token out, whatever its values.  offsets: sequences + 1 non-decreasing
+ * 4- or 8-byte integers (offset_bytes); sequence q holds the tokens
+ * [offsets[q], offsets[q+1]); tokens that no sequence holds are left out.
+ * Work arrays (`ws`, 16-byte aligned, of the bytes that the _ws_bytes
+ * function gives) need no initialisation and are free again when the call's
+ * work on `stream` is done.  Results do not depend on the order in which
+ * blocks run. */
+
+/* logp[i] = log softmax(z_i)[label_i], lse[i] = log sum exp z_i and, where
+ * `entropy` is not NULL, entropy[i] = -sum_j p_ij log p_ij. */
+int wgb_label_logprobs(const void *logits, int32_t dtype, int64_t rows,
+                       int64_t classes, int64_t row_stride, const void *labels,
+                       int32_t label_bytes, float temperature, float *logp,
+                       float *lse, float *entropy, void *stream);
+
+/* grad[i][j] = (grad_logp[i] ([j = label_i] - p_ij) - grad_entropy[i] p_ij
+ * (log p_ij + entropy[i])) / temperature, in the logits' dtype, rounded once.
+ * grad_entropy may be NULL.  `grad` may be `logits` itself (same strides). */
+int wgb_label_logprobs_grad(const void *logits, int32_t dtype, int64_t rows,
+                            int64_t classes, int64_t row_stride,
+                            const void *labels, int32_t label_bytes,
+                            float temperature, const float *lse,
+                            const float *grad_logp, const float *entropy,
+                            const float *grad_entropy, void *grad,
+                            int64_t grad_stride, void *stream);
+
+/* Preference loss.  D_q = sum (average: mean) over the kept tokens of sequence
+ * q of logp - ref_logp (ref_logp NULL: of logp); offsets NULL: every row is a
+ * sequence.  Pair p prefers sequence chosen[p] to rejected[p] (4- or 8-byte
+ * indices); x = D_chosen - D_rejected, h = beta x, and its loss is
+ *   kind 0  -(1 - smoothing) log sigmoid(h) - smoothing log sigmoid(-h)
+ *   kind 1  max(0, 1 - h)
+ *   kind 2  (x - 1 / (2 beta))^2
+ * loss = sum_p weight[p] loss_p / pairs (weight NULL: ones; no pairs: 0).
+ * grad_logp[t] = d loss / d logp[t]; chosen_reward[p] = beta D_chosen,
+ * rejected_reward[p] = beta D_rejected.  Sums of 2^40 or more count as
+ * infinite; a pair with an index out of range makes the loss NaN. */
+int64_t wgb_preference_ws_bytes(int64_t sequences, int32_t ragged);
+int wgb_preference_loss(const float *logp, const float *ref_logp,
+                        int64_t tokens, const void *offsets,
+                        int32_t offset_bytes, int64_t sequences,
+                        const uint8_t *mask, const void *chosen,
+                        const void *rejected, int32_t index_bytes,
+                        int64_t pairs, const float *weight, int32_t kind,
+                        float beta, float smoothing, int32_t average, void *ws,
+                        int64_t ws_bytes, float *loss, float *grad_logp,
+                        float *chosen_reward, float *rejected_reward,
+                        void *stream);
+
+/* Clipped policy loss with a KL term.  u = logp - old_logp, A the advantage of
+ * the token (adv_by_sequence: of its sequence).  A token is clipped where A >
+ * 0 and u > log(1 + clip_high), or A < 0 and u < log(1 - clip_low); its policy
+ * term is -A e^u, or -A (1 + clip_high) / -A (1 - clip_low) where clipped (no
+ * gradient there).  With d = ref_logp - logp its KL term is -d (kl_kind 1),
+ * d^2 / 2 (2) or e^d - 1 - d (3); ref_logp NULL: none.
+ *   loss = sum_t w_t (policy_t + kl_coef kl_t),
+ * w_t = 1 / kept tokens, or by_sequence 1 / (sequences with kept tokens *
+ * kept tokens of the sequence).  stats[5] = loss and the weighted means of
+ * the policy term, the KL term, the entropy (0 here) and the share clipped.
+ * grad_logp[t] = d loss / d logp[t].  offsets are read only where
+ * adv_by_sequence or by_sequence is set. */
+int64_t wgb_policy_ws_bytes(int64_t tokens, int64_t sequences,
+                            int32_t rows_of_logits);
+int wgb_policy_loss(const float *logp, const float *old_logp,
+                    const float *advantages, const float *ref_logp,
+                    int64_t tokens, const uint8_t *mask, const void *offsets,
+                    int32_t offset_bytes, int64_t sequences,
+                    int32_t adv_by_sequence, int32_t by_sequence,
+                    float clip_low, float clip_high, int32_t kl_kind,
+                    float kl_coef, void *ws, int64_t ws_bytes, float *stats,
+                    float *grad_logp, void *stream);
+
+/* The same from the logits, tokens = rows: logp[i] as wgb_label_logprobs gives
+ * it, loss with - entropy_coef * entropy added to each token's term, and
+ * grad[i][j] = grad_scale * d loss / d logits[i][j] in the logits' dtype,
+ * rounded once (grad_scale keeps small gradients above a 16-bit type's
+ * smallest values).  Rows that are left out have a gradient of zeros and logp
+ * 0.  `grad` may be `logits` itself (same strides). */
+int wgb_policy_loss_logits(const void *logits, int32_t dtype, int64_t rows,
+                           int64_t classes, int64_t row_stride,
+                           const void *labels, int32_t label_bytes,
+                           float temperature, const float *old_logp,
+                           const float *advantages, const float *ref_logp,
+                           const uint8_t *mask, const void *offsets,
+                           int32_t offset_bytes, int64_t sequences,
+                           int32_t adv_by_sequence, int32_t by_sequence,
+                           float clip_low, float clip_high, int32_t kl_kind,
+                           float kl_coef, float entropy_coef, float grad_scale,
+                           void *ws, int64_t ws_bytes, float *stats,
+                           float *logp, void *grad, int64_t grad_stride,
+                           void *stream);
 
 #ifdef __cplusplus
 }

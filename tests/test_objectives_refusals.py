@@ -1,0 +1,173 @@
+"""What the log-probability objectives refuse: argument checks of the Python
+calls and of the C entry points, all before any device work (no GPU)."""
+import pytest
+import torch
+
+from warpgbm_b200 import _lib
+from warpgbm_b200 import objectives as obj
+
+
+class FakeCuda(torch.Tensor):
+    """A CPU tensor that says it lies on a GPU: the checks look no further."""
+    @property
+    def device(self):
+        return torch.device("cuda", 0)
+
+
+def cuda(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(FakeCuda)
+
+
+def test_logits_are_checked():
+    y = cuda(4, dtype=torch.int64)
+    with pytest.raises(TypeError, match="logits must be a torch.Tensor"):
+        obj.label_logprobs([[1.0]], y)
+    with pytest.raises(ValueError, match="logits must be a CUDA tensor"):
+        obj.label_logprobs(torch.zeros(4, 3), y)
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        obj.label_logprobs(cuda(4, 3, dtype=torch.float64), y)
+    with pytest.raises(ValueError, match="2-dimensional"):
+        obj.label_logprobs(cuda(4), y)
+    with pytest.raises(ValueError, match="at least one class"):
+        obj.label_logprobs(cuda(4, 0), y)
+    with pytest.raises(ValueError, match="unit stride along its classes"):
+        obj.label_logprobs(cuda(3, 4).t(), y)
+    with pytest.raises(ValueError, match="must not overlap"):
+        obj.label_logprobs(cuda(1, 3).expand(4, 3), y)
+
+
+@pytest.mark.parametrize("labels,exc,msg", [
+    (cuda(4), TypeError, "labels must be torch.int32 or torch.int64"),
+    (cuda(5, dtype=torch.int64), ValueError, "labels must be 1-dimensional with 4 values"),
+    (cuda(4, 1, dtype=torch.int64), ValueError, "labels must be 1-dimensional"),
+    (torch.zeros(4, dtype=torch.int64), ValueError, "labels must be on cuda:0"),
+    (cuda(8, dtype=torch.int32)[::2], ValueError, "labels must be contiguous"),
+])
+def test_labels_are_checked(labels, exc, msg):
+    with pytest.raises(exc, match=msg):
+        obj.label_logprobs(cuda(4, 3), labels)
+
+
+@pytest.mark.parametrize("t", [0.0, -1.0, float("inf"), float("nan")])
+def test_temperature_is_checked(t):
+    with pytest.raises(ValueError, match="temperature must be positive and finite"):
+        obj.label_logprobs(cuda(4, 3), cuda(4, dtype=torch.int64), temperature=t)
+
+
+def test_gradient_buffers_are_checked():
+    x, y, v = cuda(4, 3), cuda(4, dtype=torch.int64), cuda(4)
+    with pytest.raises(ValueError, match="given together"):
+        obj.label_logprobs_grad(x, y, v, v, entropy=v)
+    with pytest.raises(ValueError, match="dtype, shape and device"):
+        obj.label_logprobs_grad(x, y, v, v, out=cuda(4, 3, dtype=torch.float16))
+    with pytest.raises(ValueError, match="dtype, shape and device"):
+        obj.label_logprobs_grad(x, y, v, v, out=cuda(4, 4))
+    base = cuda(5, 3)
+    with pytest.raises(ValueError, match="logits itself or not overlap"):
+        obj.label_logprobs_grad(base[:4], y, v, v, out=base[1:])
+    with pytest.raises(TypeError, match="grad_logp must be torch.float32"):
+        obj.label_logprobs_grad(x, y, v, cuda(4, dtype=torch.bfloat16))
+
+
+PAIRS = cuda(2, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("args,kw,exc,msg", [
+    (([1.0], PAIRS, PAIRS), {}, TypeError, "logp must be a torch.Tensor"),
+    ((torch.zeros(4), PAIRS, PAIRS), {}, ValueError, "logp must be a CUDA tensor"),
+    ((cuda(4, dtype=torch.float16), PAIRS, PAIRS), {}, TypeError, "logp must be torch.float32"),
+    ((cuda(4), PAIRS, cuda(3, dtype=torch.int32)), {}, ValueError, "rejected must be 1-dimensional with 2 values"),
+    ((cuda(4), PAIRS, cuda(2, dtype=torch.int64)), {}, TypeError, "rejected must be torch.int32"),
+    ((cuda(4), PAIRS, PAIRS), dict(beta=0.0), ValueError, "beta must be positive"),
+    ((cuda(4), PAIRS, PAIRS), dict(loss="other"), ValueError, "loss must be one of"),
+    ((cuda(4), PAIRS, PAIRS), dict(label_smoothing=0.5), ValueError, "label_smoothing must be in"),
+    ((cuda(4), PAIRS, PAIRS), dict(label_smoothing=0.1, loss="hinge"), ValueError, "for the sigmoid loss"),
+    ((cuda(4), PAIRS, PAIRS), dict(mask=cuda(4, dtype=torch.bool)), ValueError, "need offsets"),
+    ((cuda(4), PAIRS, PAIRS), dict(average=True), ValueError, "need offsets"),
+    ((cuda(4), PAIRS, PAIRS), dict(offsets=cuda(0, dtype=torch.int64)), ValueError, "one value more"),
+    ((cuda(4), PAIRS, PAIRS), dict(offsets=cuda(3)), TypeError, "offsets must be torch.int32 or torch.int64"),
+    ((cuda(4), PAIRS, PAIRS), dict(ref_logp=cuda(3)), ValueError, "ref_logp must be 1-dimensional with 4 values"),
+    ((cuda(4), PAIRS, PAIRS), dict(weight=cuda(4)), ValueError, "weight must be 1-dimensional with 2 values"),
+    ((cuda(4), PAIRS, PAIRS), dict(offsets=cuda(3, dtype=torch.int64), mask=cuda(4)), TypeError, "mask must be"),
+])
+def test_preference_refusals(args, kw, exc, msg):
+    with pytest.raises(exc, match=msg):
+        obj.preference_loss(*args, **kw)
+
+
+OFF = cuda(3, dtype=torch.int64)
+
+
+@pytest.mark.parametrize("kw,exc,msg", [
+    (dict(old_logp=cuda(3)), ValueError, "old_logp must be 1-dimensional with 4 values"),
+    (dict(advantages=cuda(3)), ValueError, "advantages must be 1-dimensional with 4 values"),
+    (dict(advantages=cuda(2, 1)), ValueError, r"need offsets"),
+    (dict(advantages=cuda(4, 1), offsets=OFF), ValueError, r"shape \(4,\) or \(2, 1\)"),
+    (dict(reduction="sequence"), ValueError, "needs offsets"),
+    (dict(reduction="sum"), ValueError, "reduction must be one of"),
+    (dict(kl="k4"), ValueError, "kl must be one of"),
+    (dict(kl_coef=0.1), ValueError, "kl_coef needs ref_logp"),
+    (dict(kl_coef=float("nan"), ref_logp=cuda(4)), ValueError, "kl_coef must be finite"),
+    (dict(clip_low=1.0), ValueError, "clip_low must be in"),
+    (dict(clip_high=-0.1), ValueError, "clip_high must be"),
+    (dict(mask=cuda(4, dtype=torch.int32)), TypeError, "mask must be"),
+])
+def test_policy_refusals(kw, exc, msg):
+    base = dict(old_logp=cuda(4), advantages=cuda(4))
+    with pytest.raises(exc, match=msg):
+        obj.policy_loss(cuda(4), **{**base, **kw})
+    with pytest.raises(exc, match=msg):
+        obj.policy_loss_logits(cuda(4, 7), cuda(4, dtype=torch.int64), **{**base, **kw})
+
+
+@pytest.mark.parametrize("kw", [dict(entropy_coef=float("inf")), dict(grad_scale=float("nan"))])
+def test_policy_logits_refusals(kw):
+    with pytest.raises(ValueError, match="must be finite"):
+        obj.policy_loss_logits(cuda(4, 7), cuda(4, dtype=torch.int64), cuda(4), cuda(4), **kw)
+
+
+def _err(rc):
+    return rc, _lib.lib().wgb_last_error().decode()
+
+
+def test_c_entry_points_report_bad_arguments():
+    L = _lib.lib()
+    bad = [
+        (L.wgb_label_logprobs(None, 3, 1, 4, 4, None, 8, 1.0, None, None, None, None), "dtype"),
+        (L.wgb_label_logprobs(None, 0, 1, 0, 4, None, 8, 1.0, None, None, None, None), "class"),
+        (L.wgb_label_logprobs(None, 0, 2, 8, 4, None, 8, 1.0, None, None, None, None), "overlap"),
+        (L.wgb_label_logprobs(None, 0, 1, 4, 4, None, 8, 0.0, None, None, None, None), "temperature"),
+        (L.wgb_label_logprobs(None, 0, 1, 4, 4, None, 8, 1.0, None, None, None, None), "null"),
+        (L.wgb_label_logprobs(2, 0, 1, 4, 4, None, 8, 1.0, None, None, None, None), "aligned"),
+        (L.wgb_label_logprobs(16, 0, 1, 4, 4, None, 2, 1.0, None, None, None, None), "labels"),
+        (L.wgb_label_logprobs(16, 0, 1, 4, 4, None, 8, 1.0, None, None, None, None), "null"),
+    ]
+    for rc, word in bad[-1:]:
+        assert rc == 1 and word in L.wgb_last_error().decode()
+    assert all(rc == 1 for rc, _ in bad)
+    calls = [
+        (lambda: L.wgb_preference_loss(None, None, 4, None, 0, 3, None, None, None, 4, 0, None, 0, 0.1, 0.0, 0, None, 0,
+                                       None, None, None, None, None), "without offsets"),
+        (lambda: L.wgb_preference_loss(None, None, 4, None, 0, 4, None, None, None, 4, 0, None, 3, 0.1, 0.0, 0, None, 0,
+                                       None, None, None, None, None), "kind"),
+        (lambda: L.wgb_preference_loss(16, None, 4, None, 0, 4, None, None, None, 4, 0, None, 0, 0.1, 0.0, 0, 16, 8,
+                                       16, 16, None, None, None), "workspace too small"),
+        (lambda: L.wgb_policy_loss(16, 16, 16, None, 4, None, None, 0, 0, 0, 1, 0.2, 0.2, 3, 0.0, 16, 1 << 20, 16, 16,
+                                   None), "need offsets"),
+        (lambda: L.wgb_policy_loss(16, 16, 16, None, 4, None, None, 0, 0, 0, 0, 0.2, 0.2, 4, 0.0, 16, 1 << 20, 16, 16,
+                                   None), "kl must be"),
+        (lambda: L.wgb_policy_loss(16, 16, 16, None, 4, None, None, 0, 0, 0, 0, 0.2, 0.2, 3, 0.0, 16, 8, 16, 16,
+                                   None), "workspace too small"),
+        (lambda: L.wgb_policy_loss(16, 16, 16, None, -1, None, None, 0, 0, 0, 0, 0.2, 0.2, 3, 0.0, 16, 8, 16, 16,
+                                   None), "bad sizes"),
+    ]
+    for call, word in calls:
+        rc, msg = _err(call())
+        assert rc == 1 and word in msg, (rc, msg)
+
+
+def test_workspace_sizes_hold_what_they_name():
+    L = _lib.lib()
+    assert L.wgb_preference_ws_bytes(0, 0) > 0
+    assert L.wgb_preference_ws_bytes(1000, 1) > L.wgb_preference_ws_bytes(1000, 0) >= 24 * 1000
+    assert L.wgb_policy_ws_bytes(1000, 10, 1) >= L.wgb_policy_ws_bytes(1000, 10, 0) + 4000

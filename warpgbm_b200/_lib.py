@@ -101,6 +101,16 @@ _SIGS = {
     "wgb_quantile_edges": ([_p, _i64, _i32, _i64, _p, _i32, _p, _p, _p], _i32),
     "wgb_quantile_pass": ([_i32, _p, _i64, _i32, _i64, _i32, _p, _p, _p, _p, _p], _i32),
     "wgb_quantile_pick": ([_i32, _p, _p, _i64, _p, _i32, _i32, _p, _p, _p], _i32),
+    "wgb_label_logprobs": ([_p, _i32, _i64, _i64, _i64, _p, _i32, _f32, _p, _p, _p, _p], _i32),
+    "wgb_label_logprobs_grad": ([_p, _i32, _i64, _i64, _i64, _p, _i32, _f32, _p, _p, _p, _p, _p, _i64, _p], _i32),
+    "wgb_preference_ws_bytes": ([_i64, _i32], _i64),
+    "wgb_preference_loss": ([_p, _p, _i64, _p, _i32, _i64, _p, _p, _p, _i32, _i64, _p, _i32, _f32, _f32, _i32,
+                             _p, _i64, _p, _p, _p, _p, _p], _i32),
+    "wgb_policy_ws_bytes": ([_i64, _i64, _i32], _i64),
+    "wgb_policy_loss": ([_p, _p, _p, _p, _i64, _p, _p, _i32, _i64, _i32, _i32, _f32, _f32, _i32, _f32,
+                         _p, _i64, _p, _p, _p], _i32),
+    "wgb_policy_loss_logits": ([_p, _i32, _i64, _i64, _i64, _p, _i32, _f32, _p, _p, _p, _p, _p, _i32, _i64, _i32,
+                                _i32, _f32, _f32, _i32, _f32, _f32, _f32, _p, _i64, _p, _p, _p, _i64, _p], _i32),
 }
 
 EXPORTED = tuple(_SIGS)
@@ -147,6 +157,8 @@ _KERNELS = {
     "wgb_grow_tree": 0, "wgb_bins_feature_major": 1, "wgb_prebinned_ingest": 1,
     "wgb_bin_matrix": 1, "wgb_predict_packed": 1, "wgb_predict_heap": 1, "wgb_quantile_edges": 2, "wgb_quantile_pass": 1, "wgb_quantile_pick": 1,
     "wgb_compute_histogram3": 6, "wgb_compute_histogram3_noalloc": 6,
+    "wgb_label_logprobs": 1, "wgb_label_logprobs_grad": 1, "wgb_preference_loss": 4, "wgb_policy_loss": 5,
+    "wgb_policy_loss_logits": 5,
     "wgb_compute_split": 1, "wgb_custom_cuda_binner": 1, "wgb_predict_forest": 1,
 }
 LAUNCHES = [0]

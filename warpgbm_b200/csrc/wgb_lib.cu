@@ -7,3 +7,4 @@
 #include "wgb_noalloc.cu"
 #include "wgb_comm.cu"
 #include "wgb_decode.cu"
+#include "wgb_objectives.cu"

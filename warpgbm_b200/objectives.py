@@ -1,0 +1,373 @@
+"""Objectives on log-probabilities, with their gradients.
+
+A boosted forest is fitted to residuals: the negative gradient of a loss with
+respect to its scores.  These calls give that gradient for losses beyond
+squared error and cross-entropy, and serve any other model whose scores lie on
+the GPU:
+
+* ``label_logprobs`` / ``label_logprobs_grad`` -- log-prob of each row's label
+  under softmax(logits / temperature), log-sum-exp and entropy, and the way
+  back to the logits;
+* ``preference_loss`` -- paired log ratios (or scores) of chosen and rejected
+  sequences;
+* ``policy_loss`` -- the clipped policy loss with a KL term on token
+  log-probs; ``policy_loss_logits`` -- the same from the logits in one pass.
+
+Every call runs on the current CUDA stream of its tensors' device, returns
+without waiting for it, and raises on arguments that it does not take.  Values
+on the device are not looked at by the host: a label or index out of range
+shows as NaN in the result.  Per-token tensors are float32, one value a token;
+sequences are ranges of tokens between neighbouring ``offsets``.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_INDEX_BYTES = {torch.int32: 4, torch.int64: 8}
+_MASKS = (torch.bool, torch.uint8)
+_LOSSES = {"sigmoid": 0, "hinge": 1, "square": 2}
+_KLS = {"k1": 1, "k2": 2, "k3": 3}
+_REDUCTIONS = {"token": 0, "sequence": 1}
+
+
+class LabelLogprobs(NamedTuple):
+    logp: torch.Tensor
+    lse: torch.Tensor
+    entropy: Optional[torch.Tensor]
+
+
+class PreferenceLoss(NamedTuple):
+    loss: torch.Tensor
+    grad_logp: torch.Tensor
+    chosen_reward: torch.Tensor
+    rejected_reward: torch.Tensor
+
+
+class PolicyLoss(NamedTuple):
+    loss: torch.Tensor
+    grad_logp: torch.Tensor
+    policy: torch.Tensor
+    kl: torch.Tensor
+    clip_fraction: torch.Tensor
+
+
+class PolicyLossLogits(NamedTuple):
+    loss: torch.Tensor
+    grad_logits: torch.Tensor
+    logp: torch.Tensor
+    policy: torch.Tensor
+    kl: torch.Tensor
+    entropy: torch.Tensor
+    clip_fraction: torch.Tensor
+
+
+# ---------------------------------------------------------------------------
+# argument checks
+# ---------------------------------------------------------------------------
+
+def _vector(t, name, n, dtypes, dev):
+    """Pointer of a contiguous 1-D CUDA tensor of n values."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if t.device != dev:
+        raise ValueError(f"{name} must be on {dev}, got {t.device}")
+    if t.dim() != 1 or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{name} must be 1-dimensional" + (f" with {n} values" if n is not None else "")
+                         + f", got shape {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+_F32 = (torch.float32,)
+_INTS = (torch.int32, torch.int64)
+
+
+def _optional(t, name, n, dtypes, dev):
+    return None if t is None else _vector(t, name, n, dtypes, dev)
+
+
+def _logits(t, name="logits"):
+    """(rows, classes, row stride) of a logits matrix."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be 2-dimensional, got shape {tuple(t.shape)}")
+    n, k = t.shape
+    if k < 1:
+        raise ValueError(f"{name} must have at least one class")
+    if k > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} must have unit stride along its classes, got strides {t.stride()}")
+    stride = t.stride(0) if n > 1 else k
+    if stride < k:
+        raise ValueError(f"rows of {name} must not overlap, got strides {t.stride()}")
+    return n, k, stride
+
+
+def _grad_like(logits, stride, out):
+    """The gradient's buffer and row stride: a new one, or the caller's."""
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        return out, logits.shape[1]
+    n, k, out_stride = _logits(out, "out")
+    if out.dtype != logits.dtype or out.shape != logits.shape or out.device != logits.device:
+        raise ValueError("out must have the dtype, shape and device of logits")
+    a, b, size = logits.data_ptr(), out.data_ptr(), logits.element_size()
+    if n and not (a == b and stride == out_stride) and \
+            a < b + ((n - 1) * out_stride + k) * size and b < a + ((n - 1) * stride + k) * size:
+        raise ValueError("out must be logits itself or not overlap it")
+    return out, out_stride
+
+
+def _temperature(t):
+    t = float(t)
+    if not 0.0 < t < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, got {t}")
+    return t
+
+
+def _choice(value, name, table):
+    if value not in table:
+        raise ValueError(f"{name} must be one of {sorted(table)}, got {value!r}")
+    return table[value]
+
+
+class _On:
+    """The device of the call's tensors as the current one; cheaper than
+    torch.cuda.device where it is the current one already."""
+    __slots__ = ("dev", "ctx")
+
+    def __init__(self, dev):
+        self.dev, self.ctx = dev, None
+
+    def __enter__(self):
+        if torch.cuda.current_device() != self.dev.index:
+            self.ctx = torch.cuda.device(self.dev)
+            self.ctx.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+# ---------------------------------------------------------------------------
+# label log-probs
+# ---------------------------------------------------------------------------
+
+def label_logprobs(logits, labels, *, temperature=1.0, entropy=False) -> LabelLogprobs:
+    """Log-prob of each row's label, log-sum-exp of the row and, if asked for,
+    its entropy, under z = logits / temperature.
+
+    logits [N, K] float32, bfloat16 or float16, unit stride along classes;
+    labels [N] int32 or int64, negative to leave a row out (zeros).  A logit of
+    -inf is a masked class; a row with nothing else has logp = lse = -inf.
+    """
+    n, k, stride = _logits(logits)
+    dev = logits.device
+    y = _vector(labels, "labels", n, _INTS, dev)
+    temperature = _temperature(temperature)
+    out = torch.empty((3 if entropy else 2, n), dtype=torch.float32, device=dev).unbind(0)
+    with _On(dev) as stream:
+        _lib.call("wgb_label_logprobs", logits.data_ptr(), _DTYPES[logits.dtype], n, k, stride, y,
+                  _INDEX_BYTES[labels.dtype], temperature, out[0].data_ptr(), out[1].data_ptr(),
+                  out[2].data_ptr() if entropy else None, stream)
+    return LabelLogprobs(out[0], out[1], out[2] if entropy else None)
+
+
+def label_logprobs_grad(logits, labels, lse, grad_logp, *, temperature=1.0, entropy=None, grad_entropy=None,
+                        out=None) -> torch.Tensor:
+    """Gradient to the logits from the gradients to ``logp`` (and, with
+    ``entropy`` as label_logprobs gave it, to the entropy).  ``out`` may be the
+    logits themselves."""
+    n, k, stride = _logits(logits)
+    dev = logits.device
+    y = _vector(labels, "labels", n, _INTS, dev)
+    lse_p = _vector(lse, "lse", n, _F32, dev)
+    g = _vector(grad_logp, "grad_logp", n, _F32, dev)
+    if (entropy is None) != (grad_entropy is None):
+        raise ValueError("entropy and grad_entropy must be given together")
+    h = _optional(entropy, "entropy", n, _F32, dev)
+    gh = _optional(grad_entropy, "grad_entropy", n, _F32, dev)
+    temperature = _temperature(temperature)
+    out, out_stride = _grad_like(logits, stride, out)
+    with _On(dev) as stream:
+        _lib.call("wgb_label_logprobs_grad", logits.data_ptr(), _DTYPES[logits.dtype], n, k, stride, y,
+                  _INDEX_BYTES[labels.dtype], temperature, lse_p, g, h, gh, out.data_ptr(), out_stride, stream)
+    return out
+
+
+# ---------------------------------------------------------------------------
+# preference loss
+# ---------------------------------------------------------------------------
+
+def preference_loss(logp, chosen, rejected, *, ref_logp=None, offsets=None, mask=None, weight=None, beta=0.1,
+                    loss="sigmoid", label_smoothing=0.0, average=False) -> PreferenceLoss:
+    """Loss of pairs of sequences of which the first is preferred.
+
+    Sequence q scores D_q = sum over its kept tokens of logp - ref_logp
+    (``average``: their mean; no ``ref_logp``: of logp); without ``offsets``
+    every row of logp is a sequence of its own, a score.  With x = D_chosen -
+    D_rejected and h = beta x a pair's loss is -log sigmoid(h) ("sigmoid", with
+    ``label_smoothing`` e: -(1-e) log sigmoid(h) - e log sigmoid(-h)),
+    max(0, 1 - h) ("hinge") or (x - 1/(2 beta))^2 ("square"); ``loss`` is the
+    mean over pairs, each times its ``weight``.  chosen / rejected [P] int32 or
+    int64 index sequences, which may take part in any number of pairs.
+    """
+    if not isinstance(logp, torch.Tensor):
+        raise TypeError("logp must be a torch.Tensor")
+    if logp.device.type != "cuda":
+        raise ValueError("logp must be a CUDA tensor")
+    dev = logp.device
+    x = _vector(logp, "logp", None, _F32, dev)
+    n = logp.shape[0]
+    ref = _optional(ref_logp, "ref_logp", n, _F32, dev)
+    c = _vector(chosen, "chosen", None, _INTS, dev)
+    p = chosen.shape[0]
+    r = _vector(rejected, "rejected", p, (chosen.dtype,), dev)
+    w = _optional(weight, "weight", p, _F32, dev)
+    kind = _choice(loss, "loss", _LOSSES)
+    beta, label_smoothing = float(beta), float(label_smoothing)
+    if not 0.0 < beta < float("inf"):
+        raise ValueError(f"beta must be positive and finite, got {beta}")
+    if not 0.0 <= label_smoothing < 0.5:
+        raise ValueError(f"label_smoothing must be in [0, 0.5), got {label_smoothing}")
+    if label_smoothing and kind != 0:
+        raise ValueError("label_smoothing is for the sigmoid loss")
+    if offsets is None:
+        if mask is not None or average:
+            raise ValueError("mask and average need offsets")
+        off, off_bytes, sequences = None, 0, n
+    else:
+        off = _vector(offsets, "offsets", None, _INTS, dev)
+        if offsets.shape[0] < 1:
+            raise ValueError("offsets must have one value more than there are sequences")
+        off_bytes, sequences = _INDEX_BYTES[offsets.dtype], offsets.shape[0] - 1
+    m = _optional(mask, "mask", n, _MASKS, dev)
+    ws_bytes = _lib.lib().wgb_preference_ws_bytes(sequences, off is not None)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    out = torch.empty(1, dtype=torch.float32, device=dev)
+    grad = torch.empty(n, dtype=torch.float32, device=dev)
+    rewards = torch.empty((2, p), dtype=torch.float32, device=dev).unbind(0)
+    with _On(dev) as stream:
+        _lib.call("wgb_preference_loss", x, ref, n, off, off_bytes, sequences, m, c, r, _INDEX_BYTES[chosen.dtype], p,
+                  w, kind, beta, label_smoothing, bool(average), ws.data_ptr(), ws_bytes, out.data_ptr(),
+                  grad.data_ptr(), rewards[0].data_ptr(), rewards[1].data_ptr(), stream)
+    return PreferenceLoss(out[0], grad, rewards[0], rewards[1])
+
+
+# ---------------------------------------------------------------------------
+# policy loss
+# ---------------------------------------------------------------------------
+
+def _policy_args(n, dev, old_logp, advantages, ref_logp, offsets, mask, clip_low, clip_high, kl_coef, kl, reduction):
+    """What the two policy calls have in common, as the library takes it."""
+    old = _vector(old_logp, "old_logp", n, _F32, dev)
+    ref = _optional(ref_logp, "ref_logp", n, _F32, dev)
+    m = _optional(mask, "mask", n, _MASKS, dev)
+    by_seq = _choice(reduction, "reduction", _REDUCTIONS)
+    kind = _choice(kl, "kl", _KLS)
+    clip_low, clip_high, kl_coef = float(clip_low), float(clip_high), float(kl_coef)
+    if not 0.0 <= clip_low < 1.0:
+        raise ValueError(f"clip_low must be in [0, 1), got {clip_low}")
+    if not 0.0 <= clip_high < float("inf"):
+        raise ValueError(f"clip_high must be non-negative and finite, got {clip_high}")
+    if not abs(kl_coef) < float("inf"):
+        raise ValueError(f"kl_coef must be finite, got {kl_coef}")
+    if kl_coef and ref is None:
+        raise ValueError("kl_coef needs ref_logp")
+    off, off_bytes, sequences = None, 0, 0
+    if offsets is not None:
+        off = _vector(offsets, "offsets", None, _INTS, dev)
+        if offsets.shape[0] < 1:
+            raise ValueError("offsets must have one value more than there are sequences")
+        off_bytes, sequences = _INDEX_BYTES[offsets.dtype], offsets.shape[0] - 1
+    elif by_seq:
+        raise ValueError("reduction='sequence' needs offsets")
+    adv_by_seq = isinstance(advantages, torch.Tensor) and advantages.dim() == 2
+    if adv_by_seq:
+        if off is None:
+            raise ValueError("advantages of shape [sequences, 1] need offsets")
+        if tuple(advantages.shape) != (sequences, 1):
+            raise ValueError(f"advantages must have shape ({n},) or ({sequences}, 1), got {tuple(advantages.shape)}")
+        adv = _vector(advantages.view(-1) if advantages.is_contiguous() else advantages[:, 0], "advantages",
+                      sequences, _F32, dev)
+    else:
+        adv = _vector(advantages, "advantages", n, _F32, dev)
+    return (old, adv, ref, m, off, off_bytes, sequences, adv_by_seq, by_seq, clip_low, clip_high, kind, kl_coef)
+
+
+def policy_loss(logp, old_logp, advantages, *, ref_logp=None, offsets=None, mask=None, clip_low=0.2, clip_high=0.2,
+                kl_coef=0.0, kl="k3", reduction="token") -> PolicyLoss:
+    """Clipped policy loss with a KL term on token log-probs, and its gradient.
+
+    With ratio = exp(logp - old_logp) a token's policy term is
+    -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A); with d = ref_logp
+    - logp its KL term is -d ("k1"), d^2/2 ("k2") or e^d - 1 - d ("k3"); the
+    loss is the mean of policy + kl_coef kl over kept tokens ("token"), or the
+    mean over sequences of their means ("sequence"; sequences without kept
+    tokens do not count).  advantages: [T], or [sequences, 1] for one a
+    sequence.  ``offsets`` matter only where one of the two goes by sequence;
+    tokens that no sequence holds are then left out.
+    """
+    if not isinstance(logp, torch.Tensor):
+        raise TypeError("logp must be a torch.Tensor")
+    if logp.device.type != "cuda":
+        raise ValueError("logp must be a CUDA tensor")
+    dev = logp.device
+    x = _vector(logp, "logp", None, _F32, dev)
+    n = logp.shape[0]
+    old, adv, ref, m, off, off_bytes, sequences, adv_by_seq, by_seq, lo, hi, kind, kl_coef = _policy_args(
+        n, dev, old_logp, advantages, ref_logp, offsets, mask, clip_low, clip_high, kl_coef, kl, reduction)
+    grad = torch.empty(n, dtype=torch.float32, device=dev)
+    stats = torch.empty(5, dtype=torch.float32, device=dev)
+    with _On(dev) as stream:
+        ws_bytes = _lib.lib().wgb_policy_ws_bytes(n, sequences, 0)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        _lib.call("wgb_policy_loss", x, old, adv, ref, n, m, off, off_bytes, sequences, adv_by_seq, by_seq, lo, hi,
+                  kind, kl_coef, ws.data_ptr(), ws_bytes, stats.data_ptr(), grad.data_ptr(), stream)
+    s = stats.unbind(0)
+    return PolicyLoss(s[0], grad, s[1], s[2], s[4])
+
+
+def policy_loss_logits(logits, labels, old_logp, advantages, *, temperature=1.0, ref_logp=None, offsets=None,
+                       mask=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, kl="k3", entropy_coef=0.0,
+                       reduction="token", grad_scale=1.0, out=None) -> PolicyLossLogits:
+    """policy_loss from the logits: log-probs of ``labels`` under softmax(logits
+    / temperature), the loss with - entropy_coef * entropy added to each token's
+    term, and ``grad_scale`` times its gradient to the logits in their dtype,
+    in one pass over them.  Rows with a negative label or a false mask are left
+    out.  ``out`` may be the logits themselves.
+    """
+    n, k, stride = _logits(logits)
+    dev = logits.device
+    y = _vector(labels, "labels", n, _INTS, dev)
+    temperature = _temperature(temperature)
+    entropy_coef, grad_scale = float(entropy_coef), float(grad_scale)
+    if not (abs(entropy_coef) < float("inf") and abs(grad_scale) < float("inf")):
+        raise ValueError("entropy_coef and grad_scale must be finite")
+    old, adv, ref, m, off, off_bytes, sequences, adv_by_seq, by_seq, lo, hi, kind, kl_coef = _policy_args(
+        n, dev, old_logp, advantages, ref_logp, offsets, mask, clip_low, clip_high, kl_coef, kl, reduction)
+    out, out_stride = _grad_like(logits, stride, out)
+    logp = torch.empty(n, dtype=torch.float32, device=dev)
+    stats = torch.empty(5, dtype=torch.float32, device=dev)
+    with _On(dev) as stream:
+        ws_bytes = _lib.lib().wgb_policy_ws_bytes(n, sequences, 1)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        _lib.call("wgb_policy_loss_logits", logits.data_ptr(), _DTYPES[logits.dtype], n, k, stride, y,
+                  _INDEX_BYTES[labels.dtype], temperature, old, adv, ref, m, off, off_bytes, sequences, adv_by_seq,
+                  by_seq, lo, hi, kind, kl_coef, entropy_coef, grad_scale, ws.data_ptr(), ws_bytes, stats.data_ptr(),
+                  logp.data_ptr(), out.data_ptr(), out_stride, stream)
+    s = stats.unbind(0)
+    return PolicyLossLogits(s[0], out, logp, s[1], s[2], s[3], s[4])
