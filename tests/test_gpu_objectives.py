@@ -707,3 +707,45 @@ def test_no_host_wait_and_capturable(obj):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got.grad_logits, want.grad_logits) and torch.equal(got.loss, want.loss)
+
+
+# ---------------------------------------------------------------------------
+# more rows than blocks: what a block carries from row to row
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n,k,dtype", [(1500, 9001, torch.bfloat16), (700, 9001, torch.float32), (900, 20480, torch.float16),
+                                       (1300, 3001, torch.bfloat16), (400, 70001, torch.bfloat16), (5000, 300, torch.float16),
+                                       (3000, 1030, torch.float32), (20000, 90, torch.bfloat16)])
+def test_many_rows(obj, n, k, dtype):
+    """Every row gives what it gives alone, with rows left out in between."""
+    x = make_logits(n, n, k, dtype, pad=k % 2)
+    y = make_labels(n, n, k)
+    y[::3] = -1
+    y[7:40] = -1
+    x[11, 5], x[n // 2, 0] = math.nan, math.inf
+    g = torch.randn(n, device="cuda", generator=gen(8))
+    old = torch.full((n,), -8.0, device="cuda")
+    r = obj.label_logprobs(x, y, entropy=True)
+    grad = obj.label_logprobs_grad(x, y, r.lse, g)
+    pol = obj.policy_loss_logits(x, y, old, g, entropy_coef=0.1, grad_scale=float(n))
+    kept = y >= 0
+    w = int(kept.sum())
+    assert not r.logp[~kept].any() and not r.entropy[~kept].any()
+    assert not grad[~kept].any() and not pol.grad_logits[~kept].any() and not pol.logp[~kept].any()
+    z = x.float()
+    lp = z.log_softmax(1)
+    want = lp.gather(1, y.clamp(min=0)[:, None])[:, 0]
+    ok = kept & torch.isfinite(want)
+    # torch's float32 log-softmax and ours are both within row_tol of the definition
+    tol = 2 * torch.from_numpy(row_tol(np.ones((1, k)) * float(z[ok].abs().max()))).max().item()
+    assert float((r.logp - want)[ok].abs().max()) < tol
+    assert float((pol.logp - want)[ok].abs().max()) < tol
+    p = lp.exp()
+    wantg = -p * g[:, None]
+    wantg[torch.arange(n, device="cuda"), y.clamp(min=0)] += g
+    err = (grad.float() - wantg)[ok].abs()
+    assert float((err - (EPS[dtype] * 1.01 * wantg[ok].abs() + tol * g[ok].abs()[:, None] * 4 + TINY[dtype])).max()) <= 0
+    # the rows alone: the same arithmetic
+    for i in ok.nonzero()[:: max(1, w // 5), 0].tolist():
+        one = obj.label_logprobs(x[i:i + 1].clone(), y[i:i + 1])
+        assert abs(float(one.logp[0]) - float(r.logp[i])) < tol

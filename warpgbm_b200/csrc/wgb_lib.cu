@@ -8,3 +8,4 @@
 #include "wgb_comm.cu"
 #include "wgb_decode.cu"
 #include "wgb_objectives.cu"
+#include "wgb_logits.cu"

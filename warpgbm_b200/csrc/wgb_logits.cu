@@ -1,0 +1,1457 @@
+// Objectives on rows of logits: label log-probs, their gradient, and the policy
+// step in one pass (group 3 of include/warpgbm_b200.h).
+//
+// A row of logits is reduced to (m, s, t): m = max x, s = sum of 2^d and t =
+// sum of 2^d d over d = (x - m) c, c = log2(e) / temperature, all in fp32.
+// Then, in natural units, log s + m / temperature is the log-sum-exp, (x_y - m)
+// / temperature - log s the label's log-prob and log s - ln2 t / s the entropy.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace wgb {
+
+constexpr float LN2F = 0.693147180559945309f;
+constexpr double LOG2E = 1.44269504088896340736;
+
+// Two fp32 values in one 64-bit register pair: sm_100a adds and multiplies both
+// in one instruction.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2_make(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 f2_split(F2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// 16 bytes of logits: as fp32 and back (one rounding to nearest, on the way
+// out), and their running maximum in the type itself (`Top`; NaN is passed over).
+// `floored` raises what is below FLOOR (-inf among it) to FLOOR and keeps NaN.
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+    static constexpr int N = 4;
+    static constexpr uint32_t LOW = 0xff800000u;  // -inf
+    static constexpr bool HALF = false;
+    static constexpr float FLOOR = 0.0f;          // not used
+    using Top = float;
+    __device__ static uint4 floored(const uint4 &u) { return u; }
+    __device__ static Top top_none() { return -INFINITY; }
+    __device__ static Top top_of(const uint4 &u, Top t) {
+        return fmaxf(fmaxf(fmaxf(t, __uint_as_float(u.x)), fmaxf(__uint_as_float(u.y), __uint_as_float(u.z))),
+                     __uint_as_float(u.w));
+    }
+    __device__ static float top_value(Top t) { return t; }
+    __device__ static void unpack(const uint4 &u, F2 (&f)[2]) {
+        f[0] = f2_make(__uint_as_float(u.x), __uint_as_float(u.y));
+        f[1] = f2_make(__uint_as_float(u.z), __uint_as_float(u.w));
+    }
+    __device__ static uint4 pack(const float (&f)[4]) {
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+    __device__ static float to(float v) { return v; }
+    __device__ static float from(float f) { return f; }
+};
+template <> struct Vec<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static constexpr uint32_t LOW = 0xff80ff80u;
+    static constexpr bool HALF = true;
+    static constexpr float FLOOR = -1.2676506002282294e30f;  // -2^100
+    using Top = __nv_bfloat162;
+    __device__ static uint32_t floored(uint32_t w) {
+        uint32_t r;
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xf180f180u));
+        return r;
+    }
+    __device__ static uint4 floored(const uint4 &u) {
+        return make_uint4(floored(u.x), floored(u.y), floored(u.z), floored(u.w));
+    }
+    __device__ static __nv_bfloat162 word(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162 *>(&w); }
+    __device__ static Top top_none() { return word(LOW); }
+    __device__ static Top top_of(const uint4 &u, Top t) {
+        return __hmax2(__hmax2(__hmax2(t, word(u.x)), __hmax2(word(u.y), word(u.z))), word(u.w));
+    }
+    __device__ static float top_value(Top t) { return fmaxf(__low2float(t), __high2float(t)); }
+    __device__ static void unpack(const uint4 &u, F2 (&f)[4]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = f2_make(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    }
+    __device__ static uint4 pack(const float (&f)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ static float to(__nv_bfloat16 v) { return __bfloat162float(v); }
+    __device__ static __nv_bfloat16 from(float f) { return __float2bfloat16_rn(f); }
+};
+template <> struct Vec<__half> {
+    static constexpr int N = 8;
+    static constexpr uint32_t LOW = 0xfc00fc00u;
+    static constexpr bool HALF = true;
+    static constexpr float FLOOR = -65504.0f;
+    using Top = __half2;
+    __device__ static uint32_t floored(uint32_t w) {
+        uint32_t r;
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xfbfffbffu));
+        return r;
+    }
+    __device__ static uint4 floored(const uint4 &u) {
+        return make_uint4(floored(u.x), floored(u.y), floored(u.z), floored(u.w));
+    }
+    __device__ static __half2 word(uint32_t w) { return *reinterpret_cast<const __half2 *>(&w); }
+    __device__ static Top top_none() { return word(LOW); }
+    __device__ static Top top_of(const uint4 &u, Top t) {
+        return __hmax2(__hmax2(__hmax2(t, word(u.x)), __hmax2(word(u.y), word(u.z))), word(u.w));
+    }
+    __device__ static float top_value(Top t) { return fmaxf(__low2float(t), __high2float(t)); }
+    __device__ static void unpack(const uint4 &u, F2 (&f)[4]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 p = __half22float2(word(w[i]));
+            f[i] = f2_make(p.x, p.y);
+        }
+    }
+    __device__ static uint4 pack(const float (&f)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ static float to(__half v) { return __half2float(v); }
+    __device__ static __half from(float f) { return __float2half_rn(f); }
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// ------------------------------------------------------------ row sums --
+struct RowSum {
+    float m, s, t;
+};
+__device__ __forceinline__ RowSum row_none() { return RowSum{-INFINITY, 0.0f, 0.0f}; }
+
+// A maximum that is subtracted: a row that is all -inf keeps exponents of -inf.
+__device__ __forceinline__ float finite_top(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// Stands in for d in products with 2^d: below it 2^d is zero, and zero times
+// -inf must be zero.
+constexpr float D_FLOOR = -1000.0f;
+
+// Moves the sums of `a` to the maximum `m` >= a.m.
+template <bool ENT>
+__device__ __forceinline__ void row_shift(RowSum &a, float m, float c) {
+    const float d = (a.m - finite_top(m)) * c;  // -inf where a holds nothing
+    const float f = exp2_fast(d);
+    if (ENT) a.t = f * fmaf(a.s, fmaxf(d, D_FLOOR), a.t);
+    a.s *= f;
+    a.m = m;
+}
+
+// Sums over W neighbouring lanes; every lane gets them.
+template <int W, bool ENT>
+__device__ __forceinline__ RowSum lanes_join(RowSum a, float c) {
+    float m = a.m;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    row_shift<ENT>(a, m, c);
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        if (ENT) a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
+    }
+    return a;
+}
+
+__device__ __forceinline__ unsigned cluster_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// mbarriers: the arrivals and the bytes of the copies that they expect complete a
+// phase.  No wait is without end: WAIT_LIMIT tries, then the caller goes on
+// with values that it marks as lost.
+constexpr int WAIT_LIMIT = 1 << 20;
+__device__ __forceinline__ void bar_init(uint64_t *bar, unsigned arrivals) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"((unsigned)__cvta_generic_to_shared(bar)), "r"(arrivals) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"((unsigned)__cvta_generic_to_shared(bar)) : "memory");
+}
+// Arrives at the same barrier of block `rank` of the cluster.
+__device__ __forceinline__ void bar_arrive_at(uint64_t *bar, unsigned rank) {
+    unsigned there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"((unsigned)__cvta_generic_to_shared(bar)), "r"(rank));
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(there) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t *bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"((unsigned)__cvta_generic_to_shared(bar)),
+                 "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t *bar, unsigned parity) {
+    unsigned ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"((unsigned)__cvta_generic_to_shared(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ void bar_wait(uint64_t *bar, unsigned parity, bool &lost) {
+    int tries = 0;
+    while (!lost && !bar_try(bar, parity)) lost = ++tries > WAIT_LIMIT;
+}
+// Writes v to the variable `mine` of block `rank` of the cluster and counts its
+// 16 bytes at that block's `bar` (only in kernels that are launched as clusters).  Unlike a barrier of the cluster this does
+// not wait for the gradients that the block has stored before.
+__device__ __forceinline__ void cluster_put(float4 *mine, uint64_t *bar, unsigned rank, const float4 &v) {
+    unsigned there, bar_there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"((unsigned)__cvta_generic_to_shared(mine)), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar_there) : "r"((unsigned)__cvta_generic_to_shared(bar)), "r"(rank));
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(there),
+                 "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(bar_there)
+                 : "memory");
+}
+
+// Sums over the warps' entries of part.
+template <int NP, bool ENT>
+__device__ __forceinline__ RowSum entries_join(const float4 *part, float c) {
+    const int lane = threadIdx.x & 31;
+    RowSum b = row_none();
+    if constexpr (NP <= 32) {
+        if (lane < NP) b = RowSum{part[lane].x, part[lane].y, part[lane].z};
+    } else {
+#pragma unroll
+        for (int i = 0; i < NP / 32; ++i) b.m = fmaxf(b.m, part[lane + 32 * i].x);
+#pragma unroll
+        for (int i = 0; i < NP / 32; ++i) {
+            RowSum e{part[lane + 32 * i].x, part[lane + 32 * i].y, part[lane + 32 * i].z};
+            row_shift<ENT>(e, b.m, c);
+            b.s += e.s;
+            if (ENT) b.t += e.t;
+        }
+    }
+    return lanes_join<32, ENT>(b, c);
+}
+
+// Sums over a group: GL <= 32 lanes, or the NT threads of a block.  `part`
+// holds NT / 32 entries and must not be the one of the previous call (its
+// readers may still be at it).
+template <int GL, int NT, bool ENT>
+__device__ __forceinline__ RowSum group_join(RowSum a, float c, float4 *part) {
+    a = lanes_join<(GL < 32 ? GL : 32), ENT>(a, c);
+    if constexpr (GL > 32) {
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_float4(a.m, a.s, a.t, 0.0f);
+        __syncthreads();
+        a = entries_join<NT / 32, ENT>(part, c);
+    }
+    return a;
+}
+// -------------------------------------------------------- 16-byte words --
+// A row is handled in words of N elements.  Word q holds the elements q N - s
+// to q N - s + N - 1, with s such that the words lie on 16-byte boundaries of
+// the row that is written (of the row itself where nothing is written).  Words
+// that reach over an end of the row are loaded and stored by elements.
+template <typename T, typename J /* int where a row's elements can be counted in one */>
+struct RowWords {
+    const T *row;
+    J K;
+    int s;    // elements of word 0 in front of the row
+    int rel;  // elements from a 16-byte boundary of `row` to a word of it
+
+    __device__ __forceinline__ RowWords(const T *r, const T *aligned_as, J k) : row(r), K(k) {
+        constexpr int N = Vec<T>::N;
+        s = (int)((reinterpret_cast<uintptr_t>(aligned_as) / sizeof(T)) % N);
+        rel = ((int)((reinterpret_cast<uintptr_t>(r) / sizeof(T)) % N) - s + N) % N;
+    }
+    __device__ __forceinline__ J words() const { return (K + s + Vec<T>::N - 1) / Vec<T>::N; }
+
+    // Whether word q can be loaded as a whole: aligned, by one load; else out of
+    // the two aligned words that it lies across.
+    __device__ __forceinline__ bool whole(J q) const {
+        constexpr int N = Vec<T>::N;
+        const J j = q * N - s;
+        return rel == 0 ? j >= 0 && j + N <= K : j >= rel && j - rel + 2 * N <= K;
+    }
+    __device__ __forceinline__ uint4 load_aligned(J q) const {
+        return *reinterpret_cast<const uint4 *>(row + (q * Vec<T>::N - s));
+    }
+    __device__ __forceinline__ uint4 load_across(J q) const {
+        const uint4 *p = reinterpret_cast<const uint4 *>(row + (q * Vec<T>::N - s - rel));
+        const uint4 lo = p[0], hi = p[1];
+        uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        const int bytes = rel * (int)sizeof(T);
+        if (bytes & 8) {
+#pragma unroll
+            for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+        }
+        if (bytes & 4) {
+#pragma unroll
+            for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+        }
+        const int bits = (bytes & 3) * 8;
+        return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                          __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+    }
+    __device__ __forceinline__ uint4 load_elements(J q) const {
+        constexpr int N = Vec<T>::N;
+        const J j = q * N - s;
+        uint4 v = make_uint4(Vec<T>::LOW, Vec<T>::LOW, Vec<T>::LOW, Vec<T>::LOW);
+        T e[N];
+        memcpy(e, &v, 16);
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (j + k >= 0 && j + k < K) e[k] = row[j + k];
+        memcpy(&v, e, 16);
+        return v;
+    }
+    // Words q0, q0 + step ... below `words`, `per` <= U of them, -inf in the
+    // place of those that are not there.  The whole ones are all under way
+    // before the first is waited for; only the rare ends take a branch.
+    template <int U>
+    __device__ __forceinline__ void load(uint4 (&w)[U], J q0, int step, int per, J words) const {
+        constexpr uint32_t L = Vec<T>::LOW;
+        bool ends = false;
+        if (rel == 0) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const J q = q0 + u * step;
+                w[u] = make_uint4(L, L, L, L);
+                if (u < per && whole(q)) w[u] = load_aligned(q);
+                else if (u < per && q < words) ends = true;
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const J q = q0 + u * step;
+                w[u] = make_uint4(L, L, L, L);
+                if (u < per && whole(q)) w[u] = load_across(q);
+                else if (u < per && q < words) ends = true;
+            }
+        }
+        if (ends) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const J q = q0 + u * step;
+                if (u < per && q < words && !whole(q)) w[u] = load_elements(q);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T *out, J q, const uint4 &v) const {
+        constexpr int N = Vec<T>::N;
+        const J j = q * N - s;
+        if (j >= 0 && j + N <= K) {
+            *reinterpret_cast<uint4 *>(out + j) = v;
+            return;
+        }
+        T e[N];
+        memcpy(e, &v, 16);
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (j + k >= 0 && j + k < K) out[j + k] = e[k];
+    }
+};
+
+// Sums of a thread as pairs.  float: d = (x - m) c with m the maximum so far.
+// 16-bit types have half the time for an element, so there d = x c - m in one
+// operation with m = x c of a large x, rounded, in the units of d (every d is
+// taken from the same m, so its rounding cancels), and with an entropy the words
+// come floored, so that no d is -inf.  That form is right while FLOOR / 2 < m / c
+// and nothing overflows (`plain`); other rows are summed again with care.
+template <typename T, bool ENT>
+struct Share {
+    float m;
+    F2 s, t;
+    __device__ __forceinline__ Share() : m(-INFINITY), s(f2_make(0.0f, 0.0f)), t(f2_make(0.0f, 0.0f)) {}
+    __device__ __forceinline__ RowSum sum() const {
+        const float2 s2 = f2_split(s), t2 = f2_split(t);
+        return RowSum{m, s2.x + s2.y, ENT ? t2.x + t2.y : 0.0f};
+    }
+    __device__ __forceinline__ void raise(float to, float unit) {
+        if (to > m) {
+            RowSum x = sum();
+            row_shift<ENT>(x, to, unit);
+            m = to;
+            s = f2_make(x.s, 0.0f);
+            t = f2_make(x.t, 0.0f);
+        }
+    }
+    template <int U>
+    __device__ __forceinline__ void add(const uint4 *w, float c) {
+        // 16 bits: once m is a maximum of real logits it stays, and 2^d may pass
+        // 1; a row that grows beyond 2^127 of it is not plain
+        if (!Vec<T>::HALF || !(m > 0.5f * Vec<T>::FLOOR * c)) {
+            typename Vec<T>::Top top = Vec<T>::top_none();
+#pragma unroll
+            for (int u = 0; u < U; ++u) top = Vec<T>::top_of(w[u], top);
+            raise(Vec<T>::HALF ? Vec<T>::top_value(top) * c : Vec<T>::top_value(top), Vec<T>::HALF ? 1.0f : c);
+        }
+        const float ft = finite_top(m);
+        const F2 mt = f2_make(-ft, -ft), c2 = f2_make(c, c);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            F2 f[Vec<T>::N / 2];
+            Vec<T>::unpack(w[u], f);
+#pragma unroll
+            for (int k = 0; k < Vec<T>::N / 2; ++k) {
+                const F2 d2 = Vec<T>::HALF ? f2_fma(f[k], c2, mt) : f2_mul(f2_add(f[k], mt), c2);
+                const float2 d = f2_split(d2);
+                const F2 e = f2_make(exp2_fast(d.x), exp2_fast(d.y));
+                s = f2_add(s, e);
+                if (ENT) t = f2_fma(e, Vec<T>::HALF ? d2 : f2_make(fmaxf(d.x, D_FLOOR), fmaxf(d.y, D_FLOOR)), t);
+            }
+        }
+    }
+    __device__ __forceinline__ void add_one(float x, float c) {
+        if (x == -INFINITY) return;
+        raise(Vec<T>::HALF ? x * c : x, Vec<T>::HALF ? 1.0f : c);
+        const float ft = finite_top(m);
+        const float d = Vec<T>::HALF ? fmaf(x, c, -ft) : (x - ft) * c, e = exp2_fast(d);
+        s = f2_add(s, f2_make(e, 0.0f));
+        if (ENT) t = f2_fma(f2_make(e, 0.0f), f2_make(fmaxf(d, D_FLOOR), 0.0f), t);
+    }
+};
+template <typename T>
+__device__ __forceinline__ bool plain(const RowSum &a, float c) {
+    return !Vec<T>::HALF || (a.m > 0.5f * Vec<T>::FLOOR * c && a.m < INFINITY && a.s < INFINITY);
+}
+
+// The sums of a row, element by element, m = max x in the units of x: for rows
+// that are not `plain`.  All threads of a group call it.
+template <typename T, int GL, int NT, bool ENT>
+__device__ __noinline__ RowSum careful_sum(const T *row, long long K, int tid, float c, float4 *part) {
+    RowSum a = row_none();
+    for (long long j = tid; j < K; j += GL) {
+        const float x = Vec<T>::to(row[j]);
+        if (x > a.m) row_shift<ENT>(a, x, c);
+        const float d = (x - finite_top(a.m)) * c, e = exp2_fast(d);
+        a.s += e;
+        if (ENT) a.t = fmaf(e, fmaxf(d, D_FLOOR), a.t);
+    }
+    return group_join<GL, NT, ENT>(a, c, part);
+}
+
+// One row of gradient: d x_j = g ([j = y] - p_j) - ge p_j (log p_j + H), with
+// log2 p_j = (x_j - top) c - b (subtracting a top near the row's maximum first
+// keeps the digits).  With d = log2 p_j that is -p_j (A d + B), A = ge ln2, B =
+// ge H + g.  16-bit gradients of plain rows take d = x_j c - b2 in one
+// operation: b2 is rounded at 2^-24 of its size, far below the 2^-12 or more of
+// the gradient's own rounding.
+struct RowGrad {
+    float top, c, b, b2, g, ge, ent;
+    bool zero;     // left out, or nothing but -inf
+    bool careful;  // not plain
+};
+template <typename T, bool GE>
+__device__ __forceinline__ uint4 word_grad(const uint4 &w, const RowGrad &r, int y /* element of the label, or -1 */) {
+    constexpr int N = Vec<T>::N;
+    F2 f[N / 2];
+    float o[N];
+    Vec<T>::unpack(w, f);
+    const F2 mt = f2_make(-r.top, -r.top), c = f2_make(r.c, r.c), mb = f2_make(-r.b, -r.b), mb2 = f2_make(-r.b2, -r.b2);
+    const float na = -r.ge * LN2F, nb = -fmaf(r.ge, r.ent, r.g);
+    const F2 A = f2_make(na, na), B = f2_make(nb, nb);
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) {
+        const F2 d2 = Vec<T>::HALF ? f2_fma(f[k], c, mb2) : f2_fma(f2_add(f[k], mt), c, mb);
+        const float2 d = f2_split(d2);
+        const F2 p = f2_make(exp2_fast(d.x), exp2_fast(d.y));
+        F2 h = B;
+        if (GE) h = f2_fma(Vec<T>::HALF ? d2 : f2_make(fmaxf(d.x, D_FLOOR), fmaxf(d.y, D_FLOOR)), A, B);
+        const float2 v = f2_split(f2_mul(p, h));
+        o[2 * k] = v.x;
+        o[2 * k + 1] = v.y;
+    }
+    if (y >= 0) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (k == y) o[k] += r.g;
+    }
+    return Vec<T>::pack(o);
+}
+// One element, the same.
+template <bool GE>
+__device__ __forceinline__ float one_grad(float x, const RowGrad &r, bool label) {
+    const float d = fmaf(x - r.top, r.c, -r.b), p = exp2_fast(d);
+    const float v = -p * (GE ? fmaf(fmaxf(d, D_FLOOR), r.ge * LN2F, fmaf(r.ge, r.ent, r.g)) : r.g);
+    return r.zero ? 0.0f : label ? v + r.g : v;
+}
+// A row's gradient element by element, by threads tid, tid + n ...
+template <typename T, bool GE>
+__device__ __noinline__ void careful_grad(const T *row, T *out, long long K, int y, int tid, int n, const RowGrad &r) {
+    for (long long j = tid; j < K; j += n) out[j] = Vec<T>::from(one_grad<GE>(Vec<T>::to(row[j]), r, j == y));
+}
+template <typename T, bool GE, typename J>
+__device__ __forceinline__ void word_emit(const RowWords<T, J> &rw, T *out, J q, const uint4 &w, const RowGrad &r,
+                                          int y) {
+    const J k = (J)y - (q * Vec<T>::N - rw.s);
+    rw.store(out, q, r.zero ? make_uint4(0u, 0u, 0u, 0u)
+                            : word_grad<T, GE>(w, r, k >= 0 && k < Vec<T>::N && y < rw.K ? (int)k : -1));
+}
+
+// --------------------------------------------------------- rows, by call --
+enum RowOp { ROW_LOGP, ROW_GRAD, ROW_POLICY };
+
+struct RowsArgs {
+    const void *logits;
+    void *grad;
+    long long rows, K, stride, grad_stride;
+    Idx labels;
+    float temperature;
+    float *logp, *lse, *ent;                              // written by ROW_LOGP (logp also by ROW_POLICY)
+    const float *lse_in, *ent_in, *g_in, *ge_in;          // ROW_GRAD
+    const float *old, *adv, *ref;                         // ROW_POLICY
+    const uint8_t *mask;
+    PolicyRule rule;
+    PolicyCount cnt;
+    double *partial;
+};
+
+// Beyond this |lse| its rounding alone moves every p by more than 2^-16, and
+// ROW_GRAD sums the row again.
+constexpr float LSE_EXACT = 256.0f;
+
+// What a row brings along besides its logits.  RowRaw is what is loaded, a row
+// ahead and without looking at it, so that nothing waits for the loads.
+struct RowRaw {
+    long long y;
+    int mask, q;           // ROW_POLICY: mask byte, sequence
+    float a0, a1, a2, a3;  // ROW_GRAD: lse, g, ge, entropy; ROW_POLICY: old, advantage, reference
+};
+struct RowIn {
+    int y;  // label; K stands for all labels past the last class
+    bool kept;
+    float a0, a1, a2, a3;  // as in RowRaw; ROW_POLICY's a3: weight
+};
+template <int OP>
+__device__ __forceinline__ RowRaw row_fetch(const RowsArgs &a, long long i) {
+    RowRaw r{-1, 1, 0, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (i >= a.rows) return r;
+    r.y = a.labels.at(i);
+    if (OP == ROW_GRAD) {
+        r.a0 = a.lse_in[i];
+        r.a1 = a.g_in[i];
+        if (a.ge_in) {
+            r.a2 = a.ge_in[i];
+            r.a3 = a.ent_in[i];
+        }
+    }
+    if (OP == ROW_POLICY) {
+        if (a.mask) r.mask = a.mask[i];
+        if (a.cnt.ids) r.q = a.cnt.ids[i];
+        r.a0 = a.old[i];
+        if (!a.rule.adv_by_sequence) r.a1 = a.adv[i];
+        if (a.rule.kl_kind) r.a2 = a.ref[i];
+    }
+    return r;
+}
+// As much of it as says whether the row is looked at.
+template <int OP>
+__device__ __forceinline__ RowRaw row_seen(const RowsArgs &a, long long i) {
+    RowRaw r{-1, 1, 0, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (i >= a.rows) return r;
+    r.y = a.labels.at(i);
+    if (OP == ROW_POLICY && a.mask) r.mask = a.mask[i];
+    if (OP == ROW_POLICY && a.cnt.ids) r.q = a.cnt.ids[i];
+    return r;
+}
+__device__ __forceinline__ int label_of(const RowRaw &r, long long K) { return (int)(r.y < 0 ? -1 : r.y < K ? r.y : K); }
+__device__ __forceinline__ bool row_kept(const RowRaw &r) { return r.y >= 0 && r.mask != 0 && r.q >= 0; }
+template <int OP>
+__device__ __forceinline__ RowIn row_open(const RowsArgs &a, const RowRaw &r, float w_all) {
+    RowIn in{label_of(r, a.K), row_kept(r), r.a0, r.a1, r.a2, r.a3};
+    if (OP == ROW_POLICY) {
+        in.a3 = w_all;
+        if (in.kept && a.rule.adv_by_sequence) in.a1 = a.adv[r.q];
+        if (in.kept && a.rule.by_sequence) in.a3 = seq_weight(a.cnt, r.q);
+    }
+    return in;
+}
+__device__ __forceinline__ bool row_resum(const RowIn &r) { return r.kept && fabsf(r.a0) > LSE_EXACT && !isinf(r.a0); }
+
+// From a row's sums (ROW_GRAD: from its lse, or from sums if `summed`) to what
+// it writes and to its gradient.  `scaled`: sum.m is in the units of d.
+template <int OP, bool ENT>
+__device__ __forceinline__ RowGrad row_close(const RowsArgs &a, const RowIn &in, const RowSum &sum, bool summed, bool scaled,
+                                             float x_y, long long i, bool leader, float inv_t, float c, double *tot) {
+    RowGrad r{0.0f, c, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, !in.kept, !scaled};
+    if (OP == ROW_GRAD) {
+        r.zero = r.zero || in.a0 == -INFINITY;
+        r.g = in.y < a.K ? in.a1 * inv_t : NAN;
+        r.ge = in.a2 * inv_t;
+        r.ent = in.a3;
+        r.top = summed ? finite_top(sum.m) : in.a0 * a.temperature;
+        r.b = summed ? log2f(sum.s) : 0.0f;
+        r.b2 = in.a0 * (float)LOG2E;
+        r.careful = summed;
+        return r;
+    }
+    const bool none = sum.s == 0.0f;  // nothing but -inf
+    const float l2 = none ? 0.0f : log2f(sum.s);
+    const float d_y = scaled ? fmaf(x_y, c, -sum.m) : (x_y - sum.m) * c;
+    const float lp = !in.kept ? 0.0f : none ? -INFINITY : (d_y - l2) * LN2F;
+    const float h = !in.kept || none ? 0.0f : ENT ? (l2 - sum.t / sum.s) * LN2F : 0.0f;
+    if (leader) {
+        a.logp[i] = lp;
+        if (OP == ROW_LOGP) {
+            a.lse[i] = !in.kept ? 0.0f : none ? -INFINITY : scaled ? (sum.m + l2) * LN2F : fmaf(sum.m, inv_t, l2 * LN2F);
+            if (ENT) a.ent[i] = h;
+        }
+    }
+    if (OP == ROW_POLICY && in.kept) {
+        const PolicyTerm p = policy_term(a.rule, lp, in.a0, in.a1, in.a2);
+        const float w = in.a3, wg = w * a.rule.grad_scale * inv_t;
+        r.g = wg * (a.rule.kl_coef != 0.0f ? fmaf(a.rule.kl_coef, p.dkl, p.dpg) : p.dpg);
+        r.ge = -wg * a.rule.ent_coef;
+        r.ent = h;
+        r.top = scaled ? 0.0f : finite_top(sum.m);
+        r.b = scaled ? sum.m + l2 : l2;
+        r.b2 = sum.m + l2;
+        r.zero = none;
+        if (leader) {
+            tot[0] += (double)w * p.pg;
+            tot[1] += (double)w * p.kl;
+            tot[2] += (double)w * h;
+            tot[3] += (double)w * p.cut;
+        }
+    }
+    return r;
+}
+template <int OP>
+__device__ __forceinline__ float row_weight_all(const RowsArgs &a) {
+    return OP == ROW_POLICY && !a.rule.by_sequence ? token_weight(a.cnt) : 0.0f;
+}
+template <typename T>
+__device__ __forceinline__ float label_logit(const T *row, const RowIn &in, long long K) {
+    return in.kept && in.y < K ? Vec<T>::to(row[in.y]) : NAN;
+}
+
+// Forms the sums of rows again whose joined sums are not plain.
+template <typename T, int GL, int NT, bool ENT>
+__device__ __forceinline__ void row_mend(RowSum &sum, bool &scaled, const T *row, long long K, bool kept, int tid, float c,
+                                         float4 *part) {
+    scaled = Vec<T>::HALF;
+    if (!Vec<T>::HALF) return;
+    const bool bad = kept && !plain<T>(sum, c);
+    if (GL > 32 ? !bad : !__any_sync(0xffffffffu, bad)) return;
+    const RowSum again = careful_sum<T, GL, NT, ENT>(row, kept ? K : 0, tid, c, part);
+    if (bad) {
+        sum = again;
+        scaled = false;
+    }
+}
+
+// Rows held in registers: GL lanes, or the NT threads of a block, hold a row in
+// U words each; the maximum, the sums and the gradient come out of the
+// registers.
+template <typename T, int OP, bool ENT, int GL, int NT, int U>
+__global__ void __launch_bounds__(NT, GL > 32 ? 1024 / NT : 4) k_rows(const __grid_constant__ RowsArgs a) {
+    constexpr bool BLOCK = GL > 32;
+    constexpr int RPC = BLOCK ? 1 : NT / GL;
+    constexpr bool SENT = ENT && OP != ROW_GRAD;  // the sums have an entropy
+    __shared__ float4 part[2][BLOCK ? NT / 32 : 1], again[BLOCK ? NT / 32 : 1];
+    __shared__ double dscratch[33];
+    pdl_wait();
+    __shared__ double shared_tot[POL_STATS];  // a block's one leader keeps its totals out of the registers
+    double own_tot[POL_STATS] = {};
+    double *tot = BLOCK ? shared_tot : own_tot;
+    if (BLOCK && threadIdx.x < POL_STATS) shared_tot[threadIdx.x] = 0.0;
+    if (BLOCK) __syncthreads();
+    const T *logits = static_cast<const T *>(a.logits);
+    T *grad = static_cast<T *>(a.grad);
+    const int tid = BLOCK ? threadIdx.x : threadIdx.x % GL;
+    const float inv_t = 1.0f / a.temperature, c = (float)LOG2E * inv_t;
+    const float w_all = row_weight_all<OP>(a);
+    const long long step = (long long)gridDim.x * RPC;
+    int turn = 0;
+    const long long mine = (long long)blockIdx.x * RPC + (BLOCK ? 0 : threadIdx.x / GL);
+    RowRaw next = row_fetch<OP>(a, mine);
+    for (long long base = (long long)blockIdx.x * RPC; base < a.rows; base += step) {
+        const long long i = base + (BLOCK ? 0 : threadIdx.x / GL);
+        const bool live = i < a.rows;
+        const RowIn in = row_open<OP>(a, next, w_all);
+        const T *row = logits + (live ? i : 0) * a.stride;
+        T *out = OP == ROW_LOGP ? nullptr : grad + (live ? i : 0) * a.grad_stride;
+        const RowWords<T, int> rw(row, OP == ROW_LOGP ? row : out, (int)a.K);
+        const int words = rw.words();
+        const int per = (words + GL - 1) / GL;  // words of a thread, at most U
+        const float x_y = OP == ROW_GRAD ? 0.0f : label_logit(row, in, a.K);
+        uint4 w[U];
+        rw.load(w, tid, GL, in.kept ? per : 0, words);
+        next = row_fetch<OP>(a, i + step);
+        if (ENT) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) w[u] = Vec<T>::floored(w[u]);
+        }
+        RowSum sum = row_none();
+        bool scaled = false, summed = true, careful = false;
+        if (OP == ROW_GRAD) {
+            careful = summed = row_resum(in);
+            if (BLOCK ? summed : __any_sync(0xffffffffu, summed)) {
+                sum = careful_sum<T, GL, NT, false>(row, summed ? a.K : 0, tid, c, part[turn]);
+                turn ^= 1;
+            }
+        } else if (!BLOCK || in.kept) {
+            Share<T, SENT> sh;
+            sh.template add<U>(w, c);
+            sum = group_join<GL, NT, SENT>(sh.sum(), Vec<T>::HALF ? 1.0f : c, part[turn]);
+            turn ^= 1;
+            row_mend<T, GL, NT, SENT>(sum, scaled, row, a.K, in.kept, tid, c, again);
+            careful = Vec<T>::HALF && in.kept && !scaled;
+        }
+        const RowGrad r = row_close<OP, ENT>(a, in, sum, summed, scaled, x_y, i, live && tid == 0, inv_t, c, tot);
+        if (!BLOCK) __syncwarp();  // in place: every lane has read its row before any writes
+        if (OP != ROW_LOGP && live) {
+            if (careful) {
+                careful_grad<T, ENT>(row, out, a.K, in.y, tid, GL, r);
+            } else {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int q = tid + u * GL;
+                    if (u < per && q < words) word_emit<T, ENT>(rw, out, q, w[u], r, in.y);
+                }
+            }
+        }
+    }
+    if (OP == ROW_POLICY) {
+        if (!BLOCK) policy_partial(own_tot, dscratch, a.partial);
+        else if (threadIdx.x == 0)
+            for (int k = 0; k < POL_STATS; ++k) a.partial[(long long)blockIdx.x * POL_STATS + k] = shared_tot[k];
+    }
+}
+
+// Rows that neither of the others takes (longer than a cluster's registers, or
+// a gradient aligned otherwise than its row): a block reads its row, and for
+// the gradient reads it again, from L2 as a rule.
+template <typename T, int OP, bool ENT, int NT>
+__global__ void __launch_bounds__(NT, 2) k_rows_long(const __grid_constant__ RowsArgs a) {
+    constexpr int U = 4;
+    constexpr bool SENT = ENT && OP != ROW_GRAD;
+    __shared__ float4 part[2][NT / 32], again[NT / 32];
+    __shared__ double tot[POL_STATS];
+    pdl_wait();
+    if (threadIdx.x < POL_STATS) tot[threadIdx.x] = 0.0;
+    __syncthreads();
+    const T *logits = static_cast<const T *>(a.logits);
+    T *grad = static_cast<T *>(a.grad);
+    const int tid = threadIdx.x;
+    const float inv_t = 1.0f / a.temperature, c = (float)LOG2E * inv_t;
+    const float w_all = row_weight_all<OP>(a);
+    int turn = 0;
+    for (long long i = blockIdx.x; i < a.rows; i += gridDim.x) {
+        const RowIn in = row_open<OP>(a, row_fetch<OP>(a, i), w_all);
+        const T *row = logits + i * a.stride;
+        T *out = OP == ROW_LOGP ? nullptr : grad + i * a.grad_stride;
+        const RowWords<T, long long> rw(row, OP == ROW_LOGP ? row : out, a.K);
+        const long long words = rw.words();
+        const float x_y = OP == ROW_GRAD ? 0.0f : label_logit(row, in, a.K);
+        const bool summed = OP == ROW_GRAD ? row_resum(in) : in.kept;
+        RowSum sum = row_none();
+        bool scaled = false, careful = OP == ROW_GRAD && summed;
+        uint4 w[U];
+        auto load = [&](long long q) {
+            rw.load(w, q, NT, U, words);
+            if (ENT) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) w[u] = Vec<T>::floored(w[u]);
+            }
+        };
+        if (careful) {
+            sum = careful_sum<T, NT, NT, false>(row, a.K, tid, c, part[turn]);
+            turn ^= 1;
+        } else if (summed) {
+            Share<T, SENT> sh;
+            for (long long q = tid; q < words; q += NT * U) {
+                load(q);
+                sh.template add<U>(w, c);
+            }
+            sum = group_join<NT, NT, SENT>(sh.sum(), Vec<T>::HALF ? 1.0f : c, part[turn]);
+            turn ^= 1;
+            row_mend<T, NT, NT, SENT>(sum, scaled, row, a.K, true, tid, c, again);
+            careful = Vec<T>::HALF && !scaled;
+        }
+        const RowGrad r = row_close<OP, ENT>(a, in, sum, summed, scaled, x_y, i, tid == 0, inv_t, c, tot);
+        if (OP == ROW_LOGP) continue;
+        if (careful || r.zero) {
+            careful_grad<T, ENT>(row, out, a.K, in.y, tid, NT, r);
+        } else {
+            for (long long q0 = tid; q0 < words; q0 += NT * U) {
+                load(q0);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const long long q = q0 + (long long)u * NT;
+                    if (q < words) word_emit<T, ENT>(rw, out, q, w[u], r, in.y);
+                }
+            }
+        }
+    }
+    if (OP == ROW_POLICY && tid == 0)
+        for (int k = 0; k < POL_STATS; ++k) a.partial[(long long)blockIdx.x * POL_STATS + k] = tot[k];
+}
+
+// ------------------------------------------------------ ring of copies --
+// Copies `bytes` (a multiple of 16, both ends on 16-byte boundaries) into this
+// block's shared memory.
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, unsigned bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     (unsigned)__cvta_generic_to_shared(dst)),
+                 "l"(src), "r"(bytes), "r"((unsigned)__cvta_generic_to_shared(bar))
+                 : "memory");
+}
+
+constexpr int RING_WARPS = 8;                 // that take words
+constexpr int RING_CONS = RING_WARPS * 32;
+constexpr int RING_NT = RING_CONS + 64;       // and one that copies and one that closes rows
+template <int OP> __host__ __device__ constexpr int ring_blocks() { return OP == ROW_LOGP ? 3 : 2; }  // of an SM
+template <int OP> __host__ __device__ constexpr int ring_lane_words() { return 4; }  // of a lane in a stage
+template <int OP> __host__ __device__ constexpr int ring_stages() { return OP == ROW_LOGP ? 4 : 6; }  // 192 KB of an SM
+template <int OP> __host__ __device__ constexpr int stage_words() { return RING_CONS * ring_lane_words<OP>(); }
+template <int OP> __host__ __device__ constexpr int ring_smem() { return ring_stages<OP>() * stage_words<OP>() * 16; }
+constexpr int RING_RECS = 8;                  // at least the stages
+
+// A row on its way: which one, its aligned words, and this block's share of them.
+struct RowRec {
+    long long i;  // -1: no more rows
+    int y;        // label, as in RowIn
+    int head, words, begin, n;
+};
+template <typename T, int CL>
+__device__ __forceinline__ RowRec row_rec(const T *row, int K, long long i, int y, int rank) {
+    constexpr int N = Vec<T>::N;
+    RowRec r;
+    r.i = i;
+    r.y = y;
+    r.head = (int)((0u - (unsigned)(reinterpret_cast<uintptr_t>(row) / sizeof(T))) % N);
+    if (r.head > K) r.head = K;
+    r.words = (K - r.head) / N;
+    const int per = (r.words + CL - 1) / CL;
+    r.begin = rank * per < r.words ? rank * per : r.words;
+    r.n = r.begin + per < r.words ? per : r.words - r.begin;
+    return r;
+}
+
+// Rows streamed through shared memory by a block, or by the CL blocks of a
+// cluster, which share each row.  One warp keeps a ring of stages full with bulk
+// copies of this row and the rows to come, so that HBM stays busy while sums
+// are joined and gradients written.  RING_WARPS warps form the sums and write
+// the gradients.  One warp turns joined sums into what a row writes, a row's
+// scalars loaded a row ahead, so that the others carry no work that is the same
+// for all.  ROW_POLICY keeps a row's stages until its gradient is written, so
+// that a row is read from HBM once.
+//
+// In place a gradient is written only after the whole row is read: the row's own
+// words, its ends and the label's logit all go into what a warp puts.
+//
+// Entries of `part` and `desc` alternate between rows.  They are not written too
+// early: a warp puts its sums of row k + 2 after the gradient of row k + 1, for
+// which every warp's sums of k + 1 were there, put after reading what belongs to
+// k (ROW_POLICY); ROW_LOGP's warps wait until row k is closed, and ROW_GRAD's
+// closing warp until all have read row k's desc.  A wait that runs out makes NaN
+// of the rows from there on.
+template <typename T, int OP, bool ENT, int CL>
+__global__ void __launch_bounds__(RING_NT, ring_blocks<OP>()) k_rows_ring(const __grid_constant__ RowsArgs a) {
+    constexpr int N = Vec<T>::N;
+    constexpr int LW = ring_lane_words<OP>();
+    constexpr int SW = stage_words<OP>();
+    constexpr int S = ring_stages<OP>();
+    constexpr bool HALF = Vec<T>::HALF;
+    constexpr bool SENT = ENT && OP != ROW_GRAD;
+    static_assert(S <= RING_RECS, "a record for every stage");
+    extern __shared__ __align__(128) uint4 ring_mem[];
+    __shared__ uint64_t full[S], empty[S], joined[2], closed[2], taken[2], mended;
+    __shared__ RowRec recs[RING_RECS];
+    __shared__ float4 part[2][CL * RING_WARPS];
+    __shared__ RowGrad desc[2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            bar_init(&full[s], 1);
+            bar_init(&empty[s], RING_WARPS);
+        }
+        for (int k = 0; k < 2; ++k) {
+            bar_init(&joined[k], CL > 1 ? 1 : RING_WARPS);
+            if (CL > 1) bar_expect(&joined[k], CL * RING_WARPS * 16);
+            bar_init(&closed[k], 1);
+            bar_init(&taken[k], RING_WARPS);
+        }
+        bar_init(&mended, CL);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async;" ::: "memory");
+    }
+    if (CL > 1) cluster_sync();
+    else __syncthreads();
+    pdl_wait();
+    const T *logits = static_cast<const T *>(a.logits);
+    T *grad = static_cast<T *>(a.grad);
+    const int K = (int)a.K;
+    const int rank = CL > 1 ? (int)cluster_rank() : 0;
+    const float inv_t = 1.0f / a.temperature, c = (float)LOG2E * inv_t;
+    const long long row0 = blockIdx.x / CL, step = gridDim.x / CL;
+    bool lost = false;
+
+    if (warp == RING_WARPS) {  // ------------------------------------ copies
+        RowRaw after = row_seen<OP>(a, row0);
+        int slot = 0, k = 0;
+        unsigned round = 0;  // times the ring has gone round
+        auto next_slot = [&]() {
+            if (++slot == S) {
+                slot = 0;
+                ++round;
+            }
+        };
+        for (long long i = row0; i < a.rows && !lost; i += step) {
+            const bool kept = row_kept(after);
+            const int y = label_of(after, a.K);
+            after = row_seen<OP>(a, i + step);
+            if (!kept) continue;
+            const T *row = logits + i * a.stride;
+            const RowRec r = row_rec<T, CL>(row, K, i, y, rank);
+            const T *src = row + r.head + (long long)r.begin * N;
+            for (int at = 0; at < r.n; at += SW) {
+                if (round) bar_wait(&empty[slot], (round - 1) & 1, lost);
+                if (lost) break;
+                if (lane == 0) {
+                    const unsigned bytes = 16u * (r.n - at < SW ? r.n - at : SW);
+                    if (at == 0) recs[k % RING_RECS] = r;
+                    bar_expect(&full[slot], bytes);
+                    bulk_load(ring_mem + slot * SW, src + (long long)at * N, bytes, &full[slot]);
+                }
+                next_slot();
+            }
+            ++k;
+        }
+        if (round && !lost) bar_wait(&empty[slot], (round - 1) & 1, lost);
+        if (lane == 0 && !lost) {
+            recs[k % RING_RECS].i = -1;
+            bar_arrive(&full[slot]);
+        }
+    } else if (warp == RING_WARPS + 1) {  // -------------------------- closing
+        const float w_all = row_weight_all<OP>(a);
+        double tot[POL_STATS] = {};
+        RowRaw next = row_fetch<OP>(a, row0);
+        int k = 0;
+        unsigned mends = 0;
+        // ROW_LOGP: rank 0 closes for the whole cluster
+        for (long long i = OP == ROW_LOGP && rank > 0 ? a.rows : row0; i < a.rows; i += step) {
+            const RowIn in = row_open<OP>(a, next, w_all);
+            next = row_fetch<OP>(a, i + step);
+            const T *row = logits + i * a.stride;
+            T *out = OP == ROW_LOGP ? nullptr : grad + i * a.grad_stride;
+            const RowRec rec = row_rec<T, CL>(row, K, i, in.y, rank);
+            float x_y = 0.0f;
+            RowSum sum = row_none();
+            bool scaled = false;
+            const bool resum = OP == ROW_GRAD && row_resum(in);
+            if (in.kept && OP != ROW_GRAD) {
+                bar_wait(&joined[k & 1], (k >> 1) & 1, lost);
+                sum = entries_join<CL * RING_WARPS, SENT>(part[k & 1], HALF ? 1.0f : c);
+                x_y = part[k & 1][0].w;
+                scaled = HALF;
+                if (lost) sum.s = NAN;
+            }
+            if (!lost && (resum || (HALF && in.kept && OP != ROW_GRAD && !plain<T>(sum, c)))) {
+                sum = careful_sum<T, 32, 32, SENT>(row, K, lane, c, nullptr);
+                scaled = false;
+                if (CL > 1 && OP != ROW_LOGP) {  // in place: every block has read the row
+                    __syncwarp();
+                    if (lane < CL) bar_arrive_at(&mended, lane);
+                    bar_wait(&mended, mends & 1, lost);
+                    ++mends;
+                }
+            }
+            RowGrad r = row_close<OP, ENT>(a, in, sum, OP != ROW_GRAD || resum, scaled, x_y, i, rank == 0 && lane == 0, inv_t,
+                                           c, tot);
+            r.careful = resum || (HALF && in.kept && OP != ROW_GRAD && !scaled);
+            if (lost) r.b = r.b2 = NAN;
+            if (in.kept) {
+                if (OP == ROW_GRAD && k >= 2) bar_wait(&taken[k & 1], ((k >> 1) - 1) & 1, lost);
+                __syncwarp();  // all lanes have read the entries
+                if (CL > 1 && OP != ROW_GRAD && lane == 0) bar_expect(&joined[k & 1], CL * RING_WARPS * 16);  // of row k + 2
+                __syncwarp();
+                if (OP == ROW_LOGP && CL > 1) {
+                    if (lane < CL) bar_arrive_at(&closed[k & 1], lane);
+                } else if (lane == 0) {
+                    if (OP != ROW_LOGP) desc[k & 1] = r;
+                    bar_arrive(&closed[k & 1]);
+                }
+                ++k;
+            }
+            if (OP != ROW_LOGP) {
+                if (!in.kept || lost) {  // a row that is left out: zeros
+                    const float v = in.kept ? NAN : 0.0f;
+                    const float f[8] = {v, v, v, v, v, v, v, v};
+                    const uint4 z = Vec<T>::pack(*reinterpret_cast<const float(*)[N]>(f));
+                    uint4 *o = reinterpret_cast<uint4 *>(out + rec.head) + rec.begin;
+                    for (int q = lane; q < rec.n; q += 32) o[q] = z;
+                }
+                if (rank == 0) {  // the elements outside the aligned words
+                    const int tail = rec.head + rec.words * N;
+                    const int at = lane < rec.head ? lane : lane >= 16 && tail + lane - 16 < K ? tail + lane - 16 : -1;
+                    if (at >= 0 && !r.careful) {
+                        const float x = in.kept ? Vec<T>::to(row[at]) : 0.0f;
+                        out[at] = Vec<T>::from(one_grad<ENT>(x, r, at == in.y));
+                    }
+                }
+            }
+        }
+        if (OP == ROW_POLICY && lane == 0)
+            for (int j = 0; j < POL_STATS; ++j) a.partial[(long long)blockIdx.x * POL_STATS + j] = tot[j];
+    } else {  // ------------------------------------------- sums and gradients
+        int slot = 0;
+        unsigned parity = 0;
+        auto read = [&](uint4 (&w)[LW], int at, unsigned ph, int n) {
+            bar_wait(&full[at], ph, lost);
+            const uint4 *from = ring_mem + at * SW + threadIdx.x;
+            if (n >= SW) {
+#pragma unroll
+                for (int u = 0; u < LW; ++u) w[u] = from[u * RING_CONS];
+            } else {
+#pragma unroll
+                for (int u = 0; u < LW; ++u) {
+                    w[u] = make_uint4(Vec<T>::LOW, Vec<T>::LOW, Vec<T>::LOW, Vec<T>::LOW);
+                    if ((int)threadIdx.x + u * RING_CONS < n) w[u] = from[u * RING_CONS];
+                }
+            }
+        };
+        auto raise_floor = [&](uint4 (&w)[LW]) {
+            if (ENT) {
+#pragma unroll
+                for (int u = 0; u < LW; ++u) w[u] = Vec<T>::floored(w[u]);
+            }
+        };
+        auto release = [&]() {
+            __syncwarp();
+            if (lane == 0) bar_arrive(&empty[slot]);
+            if (++slot == S) {
+                slot = 0;
+                parity ^= 1u;
+            }
+        };
+        uint4 w[LW];
+        for (int k = 0;; ++k) {
+            bar_wait(&full[slot], parity, lost);
+            if (lost) break;
+            const RowRec rec = recs[k % RING_RECS];
+            if (rec.i < 0) break;
+            if (OP != ROW_GRAD) {
+                Share<T, SENT> sh;
+                float x_y = 0.0f;
+                if (rank == 0 && warp == 0) {  // the label's logit, and the elements outside the aligned words
+                    const T *row = logits + rec.i * a.stride;
+                    x_y = rec.y < K ? Vec<T>::to(row[rec.y]) : NAN;
+                    const int tail = rec.head + rec.words * N;
+                    const int at = lane < rec.head ? lane : lane >= 16 && tail + lane - 16 < K ? tail + lane - 16 : -1;
+                    if (at >= 0) sh.add_one(Vec<T>::to(row[at]), c);
+                }
+                int s = slot;
+                unsigned ph = parity;
+                for (int at = 0; at < rec.n; at += SW) {
+                    read(w, s, ph, rec.n - at);
+                    if (OP == ROW_LOGP) release();
+                    raise_floor(w);
+                    sh.template add<LW>(w, c);
+                    if (++s == S) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+                RowSum sum = lanes_join<32, SENT>(sh.sum(), HALF ? 1.0f : c);
+                if (lost) sum.s = NAN;
+                if (OP == ROW_LOGP && k >= 2) bar_wait(&closed[k & 1], ((k >> 1) - 1) & 1, lost);
+                float4 *at = &part[k & 1][rank * RING_WARPS + warp];
+                const float4 v = make_float4(sum.m, sum.s, sum.t, x_y);
+                if constexpr (CL > 1) {
+                    if (lane < (OP == ROW_LOGP ? 1 : CL)) cluster_put(at, &joined[k & 1], lane, v);
+                } else if (lane == 0) {
+                    *at = v;
+                    bar_arrive(&joined[k & 1]);
+                }
+            }
+            if (OP == ROW_LOGP) continue;
+            bar_wait(&closed[k & 1], (k >> 1) & 1, lost);
+            const RowGrad r = desc[k & 1];
+            const int y = rec.y;
+            if (OP == ROW_GRAD) {
+                __syncwarp();
+                if (lane == 0) bar_arrive(&taken[k & 1]);
+            }
+            T *out = grad + rec.i * a.grad_stride;
+            if (r.careful) {
+                careful_grad<T, ENT>(logits + rec.i * a.stride, out, K, y, rank * RING_CONS + threadIdx.x, CL * RING_CONS, r);
+                for (int at = 0; at < rec.n; at += SW) {
+                    bar_wait(&full[slot], parity, lost);
+                    release();
+                }
+                continue;
+            }
+            // this thread's first word, and the label's word from there
+            uint4 *o = reinterpret_cast<uint4 *>(out + rec.head) + rec.begin + threadIdx.x;
+            const int yq = y >= rec.head ? (y - rec.head) / N - rec.begin - (int)threadIdx.x : -1, yk = (y - rec.head) % N;
+            for (int at = 0; at < rec.n; at += SW) {
+                read(w, slot, parity, rec.n - at);
+                release();
+                raise_floor(w);
+#pragma unroll
+                for (int u = 0; u < LW; ++u) {
+                    const int q = at + u * RING_CONS;
+                    if (q + (int)threadIdx.x < rec.n)
+                        o[q] = r.zero ? make_uint4(0u, 0u, 0u, 0u) : word_grad<T, ENT>(w[u], r, q == yq ? yk : -1);
+                }
+            }
+        }
+    }
+    if (lost)  // copies that did not arrive in time may still do so
+        for (int t = 0; t < 1000; ++t) __nanosleep(1000);
+    if (CL > 1) cluster_sync();
+}
+
+// Rows of few classes: a thread to a row.  A block stages TILE_ROWS rows in
+// shared memory as fp32 (pitch odd, so that the threads' columns lie in
+// different banks), which makes the loads and stores of HBM consecutive
+// whatever the number of classes.
+constexpr int TILE_ROWS = 128;
+constexpr int TILE_CLASSES = 32;
+constexpr int TILE_BATCH = 8;  // loads in flight
+
+template <typename T, int OP, bool ENT>
+__global__ void __launch_bounds__(TILE_ROWS) k_rows_tile(const __grid_constant__ RowsArgs a) {
+    extern __shared__ float tile[];
+    __shared__ double dscratch[33];
+    pdl_wait();
+    const T *logits = static_cast<const T *>(a.logits);
+    T *grad = static_cast<T *>(a.grad);
+    const int K = (int)a.K, pitch = K | 1, tid = threadIdx.x;
+    const float inv_t = 1.0f / a.temperature, c = (float)LOG2E * inv_t;
+    const float w_all = row_weight_all<OP>(a);
+    double tot[POL_STATS] = {};
+    const int dr = TILE_ROWS / K, dc = TILE_ROWS - dr * K;  // TILE_ROWS elements on, in rows and columns
+    float *mine = tile + tid * pitch;
+    for (long long i0 = (long long)blockIdx.x * TILE_ROWS; i0 < a.rows; i0 += (long long)gridDim.x * TILE_ROWS) {
+        const int n = (int)(a.rows - i0 < TILE_ROWS ? a.rows - i0 : TILE_ROWS);
+        const long long i = i0 + tid;
+        const bool live = tid < n;
+        const RowIn in = row_open<OP>(a, row_fetch<OP>(a, live ? i : a.rows), w_all);
+        int r = tid / K, k = tid - r * K;
+        for (int e0 = 0; e0 < K; e0 += TILE_BATCH) {  // a thread moves K elements in all
+            float v[TILE_BATCH];
+            int at[TILE_BATCH];
+#pragma unroll
+            for (int e = 0; e < TILE_BATCH; ++e) {
+                at[e] = e0 + e < K && r < n ? r * pitch + k : -1;
+                if (at[e] >= 0) v[e] = Vec<T>::to(logits[(i0 + r) * a.stride + k]);
+                r += dr;
+                k += dc;
+                if (k >= K) {
+                    k -= K;
+                    ++r;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < TILE_BATCH; ++e)
+                if (at[e] >= 0) tile[at[e]] = v[e];
+        }
+        __syncthreads();
+        RowSum sum = row_none();
+        const bool summed = OP == ROW_GRAD ? row_resum(in) : in.kept;
+        if (summed) {
+            for (int j = 0; j < K; ++j) sum.m = fmaxf(sum.m, mine[j]);
+            const float top = finite_top(sum.m);
+            for (int j = 0; j < K; ++j) {
+                const float d = (mine[j] - top) * c, e = exp2_fast(d);
+                sum.s += e;
+                if (ENT && OP != ROW_GRAD) sum.t = fmaf(e, fmaxf(d, D_FLOOR), sum.t);
+            }
+        }
+        const float x_y = OP != ROW_GRAD && in.kept && in.y < K ? mine[in.y] : NAN;
+        const RowGrad g = row_close<OP, ENT>(a, in, sum, summed, false, x_y, i, live, inv_t, c, tot);
+        if (OP != ROW_LOGP) {
+            if (live) {
+                for (int j = 0; j < K; ++j) mine[j] = one_grad<ENT>(mine[j], g, j == in.y);
+            }
+            __syncthreads();
+            r = tid / K;
+            k = tid - r * K;
+            while (r < n) {
+                grad[(i0 + r) * a.grad_stride + k] = Vec<T>::from(tile[r * pitch + k]);
+                r += dr;
+                k += dc;
+                if (k >= K) {
+                    k -= K;
+                    ++r;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (OP == ROW_POLICY) policy_partial(tot, dscratch, a.partial);
+}
+
+// ---------------------------------------------------------------- host --
+static int check_logits(const void *logits, int dtype, long long rows, long long K, long long stride, float temperature) {
+    WGB_CHECK_ARG(dtype >= 0 && dtype <= 2, "logits dtype must be 0 (float32), 1 (bfloat16) or 2 (float16)");
+    WGB_CHECK_ARG(rows >= 0 && K >= 1, "logits need at least one class");
+    WGB_CHECK_ARG(K < (1ll << 31), "logits have at most 2^31 - 1 classes");
+    WGB_CHECK_ARG(rows <= 1 || stride >= K, "rows of logits overlap: stride %lld, %lld classes", stride, K);
+    WGB_CHECK_ARG(temperature > 0.0f && !isinf(temperature), "temperature must be positive and finite");
+    WGB_CHECK_ARG(rows == 0 || logits != nullptr, "logits is null");
+    const int size = dtype == 0 ? 4 : 2;
+    WGB_CHECK_ARG(reinterpret_cast<uintptr_t>(logits) % size == 0, "logits are not aligned to their type");
+    return WGB_OK;
+}
+
+// Resident clusters (or blocks) of a kernel on the current device.
+template <typename K>
+static int resident(K kernel, int nt, int cl, int smem, int (&cache)[64]) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sm_count();
+    if (!cache[dev]) {
+        int n = 0;
+        if (cl == 1) {
+            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, nt, smem) != cudaSuccess) n = 0;
+            n *= sm_count();
+        } else {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(cl);
+            cfg.blockDim = dim3(nt);
+            cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = cl;
+            at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+            cfg.attrs = at;
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
+        }
+        cache[dev] = n > 0 ? n : 1;
+    }
+    return cache[dev];
+}
+
+// Launches `kernel` over `units` rows (or tiles): one wave of persistent blocks.
+template <typename K>
+static int launch_rows(K kernel, long long units, int nt, int cl, int smem, int (&cache)[64], const RowsArgs &a, int &grid,
+                       cudaStream_t st) {
+    long long n = resident(kernel, nt, cl, smem, cache);
+    if (n * cl > (long long)sm_count() * POL_BLOCKS_PER_SM) n = (long long)sm_count() * POL_BLOCKS_PER_SM / cl;
+    grid = (int)(units < n ? units : n) * cl;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(nt);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cl;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cl > 1 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    if (e != cudaSuccess) {
+        set_error("launch of a logits kernel failed: %s", cudaGetErrorString(e));
+        return WGB_ERR_CUDA;
+    }
+    return WGB_OK;
+}
+
+template <typename T, int OP, bool ENT, int GL, int NT, int U>
+static int go_rows(const RowsArgs &a, int &grid, cudaStream_t st) {
+    static int cache[64];
+    constexpr int RPC = GL > 32 ? 1 : NT / GL;
+    return launch_rows(k_rows<T, OP, ENT, GL, NT, U>, (a.rows + RPC - 1) / RPC, NT, 1, 0, cache, a, grid, st);
+}
+
+template <typename T, int OP, bool ENT, int CL>
+static int go_ring(const RowsArgs &a, int &grid, cudaStream_t st) {
+    static int cache[64];
+    constexpr int smem = ring_smem<OP>();
+    auto kernel = k_rows_ring<T, OP, ENT, CL>;
+    int dev = 0;
+    WGB_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !cache[dev])
+        WGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    return launch_rows(kernel, a.rows, RING_NT, CL, smem, cache, a, grid, st);
+}
+
+// Which kernel takes rows of K logits: a thread a row up to 32 classes; the
+// registers of 8 or 32 lanes or of a block hold up to 32, 128 and 1024 words;
+// the ring takes longer rows.
+template <typename T, int OP, bool ENT>
+static int run_rows(const RowsArgs &a, int &grid, cudaStream_t st) {
+    constexpr int N = Vec<T>::N;
+    if (a.K <= TILE_CLASSES) {
+        static int cache[64];
+        return launch_rows(k_rows_tile<T, OP, ENT>, (a.rows + TILE_ROWS - 1) / TILE_ROWS, TILE_ROWS, 1,
+                           TILE_ROWS * ((int)a.K | 1) * (int)sizeof(float), cache, a, grid, st);
+    }
+    const long long words = (a.K + 2 * N - 2) / N;  // at most, whatever the alignment
+    if (words <= 32) return go_rows<T, OP, ENT, 8, 128, 4>(a, grid, st);
+    if (words <= 128) return go_rows<T, OP, ENT, 32, 128, 4>(a, grid, st);
+    if (words <= 1024) return go_rows<T, OP, ENT, 256, 256, 4>(a, grid, st);
+    // the ring wants the row and its gradient aligned alike
+    const bool alike = OP == ROW_LOGP || ((reinterpret_cast<uintptr_t>(a.logits) - reinterpret_cast<uintptr_t>(a.grad)) % 16 == 0 &&
+                                          (a.rows <= 1 || (a.stride - a.grad_stride) * (long long)sizeof(T) % 16 == 0));
+    if (alike && a.K < (1ll << 30)) {
+        const long long inner = a.K / N;  // whole words, at most
+        int cl = 1;
+        if (OP == ROW_POLICY)  // a third of the stages is left for the rows to come
+            while (cl < 8 && inner > (long long)cl * stage_words<OP>() * (ring_stages<OP>() * 2 / 3)) cl *= 2;
+        // few rows: more blocks to a row, while the SMs are not all taken
+        while (cl < 8 && a.rows * cl * 2 <= sm_count()) cl *= 2;
+        if (OP != ROW_POLICY || inner <= (long long)cl * stage_words<OP>() * ring_stages<OP>()) {
+            if (cl == 1) return go_ring<T, OP, ENT, 1>(a, grid, st);
+            if (cl == 2) return go_ring<T, OP, ENT, 2>(a, grid, st);
+            if (cl == 4) return go_ring<T, OP, ENT, 4>(a, grid, st);
+            return go_ring<T, OP, ENT, 8>(a, grid, st);
+        }
+    }
+    static int cache[64];
+    return launch_rows(k_rows_long<T, OP, ENT, 512>, a.rows, 512, 1, 0, cache, a, grid, st);
+}
+
+// `ent`: the call has an entropy (log-probs) or an entropy gradient.
+template <int OP>
+static int run_typed(int dtype, bool ent, const RowsArgs &a, int &grid, cudaStream_t st) {
+    if (dtype == 0) return ent ? run_rows<float, OP, true>(a, grid, st) : run_rows<float, OP, false>(a, grid, st);
+    if (dtype == 1)
+        return ent ? run_rows<__nv_bfloat16, OP, true>(a, grid, st) : run_rows<__nv_bfloat16, OP, false>(a, grid, st);
+    return ent ? run_rows<__half, OP, true>(a, grid, st) : run_rows<__half, OP, false>(a, grid, st);
+}
+
+}  // namespace wgb
+
+using namespace wgb;
+
+extern "C" int wgb_label_logprobs(const void *logits, int32_t dtype, int64_t rows, int64_t classes, int64_t row_stride,
+                                  const void *labels, int32_t label_bytes, float temperature, float *logp, float *lse,
+                                  float *entropy, void *stream) {
+    WGB_TRY(check_logits(logits, dtype, rows, classes, row_stride, temperature));
+    WGB_TRY(check_index("labels", label_bytes));
+    if (rows == 0) return WGB_OK;
+    WGB_CHECK_ARG(labels && logp && lse, "labels, logp and lse must not be null");
+    RowsArgs a = {};
+    a.logits = logits;
+    a.rows = rows;
+    a.K = classes;
+    a.stride = row_stride;
+    a.labels = Idx{labels, label_bytes == 8};
+    a.temperature = temperature;
+    a.logp = logp;
+    a.lse = lse;
+    a.ent = entropy;
+    int grid;
+    return run_typed<ROW_LOGP>(dtype, entropy != nullptr, a, grid, as_stream(stream));
+}
+
+extern "C" int wgb_label_logprobs_grad(const void *logits, int32_t dtype, int64_t rows, int64_t classes,
+                                       int64_t row_stride, const void *labels, int32_t label_bytes, float temperature,
+                                       const float *lse, const float *grad_logp, const float *entropy,
+                                       const float *grad_entropy, void *grad, int64_t grad_stride, void *stream) {
+    WGB_TRY(check_logits(logits, dtype, rows, classes, row_stride, temperature));
+    WGB_TRY(check_logits(grad, dtype, rows, classes, grad_stride, temperature));
+    WGB_TRY(check_index("labels", label_bytes));
+    if (rows == 0) return WGB_OK;
+    WGB_CHECK_ARG(labels && lse && grad_logp, "labels, lse and grad_logp must not be null");
+    WGB_CHECK_ARG(!grad_entropy || entropy, "grad_entropy needs the entropies");
+    RowsArgs a = {};
+    a.logits = logits;
+    a.grad = grad;
+    a.rows = rows;
+    a.K = classes;
+    a.stride = row_stride;
+    a.grad_stride = grad_stride;
+    a.labels = Idx{labels, label_bytes == 8};
+    a.temperature = temperature;
+    a.lse_in = lse;
+    a.g_in = grad_logp;
+    a.ent_in = entropy;
+    a.ge_in = grad_entropy;
+    int grid;
+    return run_typed<ROW_GRAD>(dtype, grad_entropy != nullptr, a, grid, as_stream(stream));
+}
+
+extern "C" int wgb_policy_loss_logits(const void *logits, int32_t dtype, int64_t rows, int64_t classes,
+                                      int64_t row_stride, const void *labels, int32_t label_bytes, float temperature,
+                                      const float *old_logp, const float *advantages, const float *ref_logp,
+                                      const uint8_t *mask, const void *offsets, int32_t offset_bytes, int64_t sequences,
+                                      int32_t adv_by_sequence, int32_t by_sequence, float clip_low, float clip_high,
+                                      int32_t kl_kind, float kl_coef, float entropy_coef, float grad_scale, void *ws,
+                                      int64_t ws_bytes, float *stats, float *logp, void *grad, int64_t grad_stride,
+                                      void *stream) {
+    WGB_TRY(check_logits(logits, dtype, rows, classes, row_stride, temperature));
+    WGB_TRY(check_logits(grad, dtype, rows, classes, grad_stride, temperature));
+    WGB_TRY(check_index("labels", label_bytes));
+    WGB_CHECK_ARG(sequences >= 0 && sequences < (1ll << 31), "too many sequences");
+    PolicyRule rule;
+    WGB_TRY(policy_rule(
+        PolicyArgs{clip_low, clip_high, kl_coef, entropy_coef, grad_scale, kl_kind, by_sequence, adv_by_sequence},
+        ref_logp, rows, rule));
+    if (offsets) WGB_TRY(check_index("offsets", offset_bytes));
+    WGB_CHECK_ARG(offsets || (!by_sequence && !adv_by_sequence), "a mean or advantages by sequence need offsets");
+    WGB_CHECK_ARG(rows == 0 || (labels && old_logp && advantages && logp),
+                  "labels, old_logp, advantages and logp must not be null");
+    WGB_CHECK_ARG(stats != nullptr, "stats must not be null");
+    const bool seqs = by_sequence || adv_by_sequence;
+    WGB_CHECK_ARG(ws && ws_bytes >= wgb_policy_ws_bytes(rows, sequences, 1), "workspace too small");
+    WGB_CHECK_ARG(reinterpret_cast<uintptr_t>(ws) % 16 == 0, "workspace is not aligned to 16 bytes");
+    cudaStream_t st = as_stream(stream);
+    const PolicyWs w = policy_ws(ws, rows, sequences, seqs);
+    const Idx off{seqs ? offsets : nullptr, offset_bytes == 8}, lab{labels, label_bytes == 8};
+    WGB_TRY(policy_counts(w, mask, lab, rows, off, sequences, rule, st));
+    RowsArgs a = {};
+    a.logits = logits;
+    a.grad = grad;
+    a.rows = rows;
+    a.K = classes;
+    a.stride = row_stride;
+    a.grad_stride = grad_stride;
+    a.labels = lab;
+    a.temperature = temperature;
+    a.logp = logp;
+    a.old = old_logp;
+    a.adv = advantages;
+    a.ref = ref_logp;
+    a.mask = mask;
+    a.rule = rule;
+    a.cnt = PolicyCount{w.total, w.acc, w.ids};
+    a.partial = w.partial;
+    int grid = 0;
+    if (rows) WGB_TRY(run_typed<ROW_POLICY>(dtype, true, a, grid, st));
+    WGB_PDL("k_policy_finish", k_policy_finish, dim3(1), dim3(256), 0, st, (const double *)w.partial, grid, rule, stats);
+    return WGB_OK;
+}

@@ -1,87 +1,15 @@
-// Objectives on log-probabilities: label log-probs of rows of logits and their
-// gradient, a preference loss over paired log ratios, and a clipped policy
-// loss with a KL term (group 3 of include/warpgbm_b200.h).
+// Objectives on per-token log-probabilities: a preference loss over paired log
+// ratios and a clipped policy loss with a KL term (group 3 of
+// include/warpgbm_b200.h; the calls that take rows of logits are in
+// wgb_logits.cu).
 //
-// Arithmetic.  A row of logits is reduced to (m, s, t): m = max x, s = sum of
-// 2^d and t = sum of 2^d d over d = (x - m) c, c = log2(e) / temperature, all
-// in fp32.  Then, in natural units, log s + m / temperature is the
-// log-sum-exp, (x_y - m) / temperature - log s the label's log-prob and
-// log s - ln2 t / s the entropy.  Sums over tokens are exact: a partial sum
-// formed in a fixed order is added to a 128-bit fixed-point number with
-// integer atomics (Acc), so no result depends on the order of the atomics.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+// Sums over the tokens of a sequence and over the pairs of a sequence are
+// exact: a partial sum formed in a fixed order is added to a 128-bit
+// fixed-point number with integer atomics (Acc), so no result depends on the
+// order of the atomics.
+#include <type_traits>
 
 namespace wgb {
-
-constexpr float LN2F = 0.693147180559945309f;
-constexpr double LOG2E = 1.44269504088896340736;
-
-__device__ __forceinline__ float exp2_fast(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
-// 16 bytes of logits as fp32 and back (one rounding to nearest, on the way out)
-template <typename T> struct Vec;
-template <> struct Vec<float> {
-    static constexpr int N = 4;
-    __device__ static void unpack(const uint4 &u, float (&f)[4]) {
-        f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y);
-        f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
-    }
-    __device__ static uint4 pack(const float (&f)[4]) {
-        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-    }
-    __device__ static float to(float v) { return v; }
-    __device__ static float from(float f) { return f; }
-};
-template <> struct Vec<__nv_bfloat16> {
-    static constexpr int N = 8;
-    __device__ static void unpack(const uint4 &u, float (&f)[8]) {
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f[2 * i] = __uint_as_float(w[i] << 16);
-            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    }
-    __device__ static uint4 pack(const float (&f)[8]) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t *>(&h);
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    __device__ static float to(__nv_bfloat16 v) { return __bfloat162float(v); }
-    __device__ static __nv_bfloat16 from(float f) { return __float2bfloat16_rn(f); }
-};
-template <> struct Vec<__half> {
-    static constexpr int N = 8;
-    __device__ static void unpack(const uint4 &u, float (&f)[8]) {
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-            f[2 * i] = p.x;
-            f[2 * i + 1] = p.y;
-        }
-    }
-    __device__ static uint4 pack(const float (&f)[8]) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t *>(&h);
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    __device__ static float to(__half v) { return __half2float(v); }
-    __device__ static __half from(float f) { return __float2half_rn(f); }
-};
 
 // An index array of 4- or 8-byte integers.
 struct Idx {
@@ -91,260 +19,6 @@ struct Idx {
         return wide ? static_cast<const long long *>(p)[i] : static_cast<const int *>(p)[i];
     }
 };
-
-// ------------------------------------------------------------ row sums --
-struct RowSum {
-    float m, s, t;
-};
-__device__ __forceinline__ RowSum row_empty() { return RowSum{-INFINITY, 0.0f, 0.0f}; }
-
-// A maximum that is subtracted: a row that is all -inf keeps exponents of -inf.
-__device__ __forceinline__ float finite_top(float m) { return m == -INFINITY ? 0.0f : m; }
-
-// d below every exponent that 2^d does not flush to zero, for d * 2^d terms
-// that must not be -inf * 0
-constexpr float D_FLOOR = -1000.0f;
-
-template <bool ENT>
-__device__ __forceinline__ void row_add(RowSum &a, float x, float top, float c) {
-    const float d = (x - top) * c;
-    const float e = exp2_fast(d);
-    a.s += e;
-    if (ENT) a.t = fmaf(e, fmaxf(d, D_FLOOR), a.t);
-}
-
-// Moves the sums of `a` to the maximum `m` >= a.m.
-template <bool ENT>
-__device__ __forceinline__ void row_shift(RowSum &a, float m, float c) {
-    const float d = (a.m - finite_top(m)) * c;  // -inf where a is empty
-    const float f = exp2_fast(d);
-    if (ENT) a.t = f * fmaf(a.s, fmaxf(d, D_FLOOR), a.t);
-    a.s *= f;
-    a.m = m;
-}
-
-template <bool ENT>
-__device__ __forceinline__ RowSum row_join(RowSum a, RowSum b, float c) {
-    const float m = fmaxf(a.m, b.m);
-    row_shift<ENT>(a, m, c);
-    row_shift<ENT>(b, m, c);
-    a.s += b.s;
-    if (ENT) a.t += b.t;
-    return a;
-}
-
-// Sums over the G threads of a group: a warp, or the whole block.
-template <int G, bool ENT>
-__device__ __forceinline__ RowSum group_join(RowSum a, float c, RowSum *scratch /* >= 33 */) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        RowSum b;
-        b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-        b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-        b.t = ENT ? __shfl_xor_sync(0xffffffffu, a.t, o) : 0.0f;
-        a = row_join<ENT>(a, b, c);
-    }
-    if (G > 32) {
-        const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-        if (lane == 0) scratch[w] = a;
-        __syncthreads();
-        if (w == 0) {
-            RowSum b = lane < G / 32 ? scratch[lane] : row_empty();
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                RowSum t;
-                t.m = __shfl_xor_sync(0xffffffffu, b.m, o);
-                t.s = __shfl_xor_sync(0xffffffffu, b.s, o);
-                t.t = ENT ? __shfl_xor_sync(0xffffffffu, b.t, o) : 0.0f;
-                b = row_join<ENT>(b, t, c);
-            }
-            if (lane == 0) scratch[32] = b;
-        }
-        __syncthreads();
-        a = scratch[32];
-        __syncthreads();
-    }
-    return a;
-}
-
-// Row of K elements as: `head` single elements, `vecs` aligned 16-byte words,
-// then single elements again.
-struct RowCut {
-    long long head, vecs;
-};
-template <typename T>
-__device__ __forceinline__ RowCut row_cut(const T *row, long long K) {
-    constexpr int N = Vec<T>::N;
-    const int off = (int)((reinterpret_cast<uintptr_t>(row) / sizeof(T)) % N);
-    long long head = off ? N - off : 0;
-    if (head > K) head = K;
-    return RowCut{head, (K - head) / N};
-}
-
-// (m, s, t) of this thread's share of a row.
-template <typename T, int G, bool ENT>
-__device__ __forceinline__ RowSum row_scan(const T *row, long long K, int tid, float c) {
-    constexpr int N = Vec<T>::N;
-    RowSum a = row_empty();
-    auto single = [&](long long j) {
-        const float x = Vec<T>::to(row[j]);
-        if (x > a.m) row_shift<ENT>(a, x, c);
-        row_add<ENT>(a, x, finite_top(a.m), c);
-    };
-    if (G <= 32) {
-        for (long long j = tid; j < K; j += G) single(j);
-        return a;
-    }
-    const RowCut cut = row_cut(row, K);
-    if (tid < cut.head) single(tid);
-    const uint4 *v = reinterpret_cast<const uint4 *>(row + cut.head);
-    constexpr int U = 4;
-    for (long long i = tid; i < cut.vecs; i += (long long)G * U) {
-        uint4 w[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i + (long long)u * G < cut.vecs) w[u] = v[i + (long long)u * G];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (i + (long long)u * G >= cut.vecs) break;
-            float f[N];
-            Vec<T>::unpack(w[u], f);
-            float m = f[0];
-#pragma unroll
-            for (int k = 1; k < N; ++k) m = fmaxf(m, f[k]);
-            if (m > a.m) row_shift<ENT>(a, m, c);
-            const float top = finite_top(a.m);
-#pragma unroll
-            for (int k = 0; k < N; ++k) row_add<ENT>(a, f[k], top, c);
-        }
-    }
-    for (long long j = cut.head + cut.vecs * N + tid; j < K; j += G) single(j);
-    return a;
-}
-
-// What a row's sums say: log-prob of the label, log-sum-exp, entropy.
-struct RowStat {
-    float logp, lse, ent, logs;
-};
-template <typename T, bool ENT>
-__device__ __forceinline__ RowStat row_stat(const RowSum &a, const T *row, long long K, long long y, float inv_t) {
-    RowStat r{-INFINITY, -INFINITY, 0.0f, 0.0f};
-    if (a.s == 0.0f) return r;  // every logit is -inf
-    r.logs = logf(a.s);
-    r.lse = fmaf(a.m, inv_t, r.logs);
-    r.logp = y < K ? fmaf(Vec<T>::to(row[y]) - a.m, inv_t, -r.logs) : NAN;
-    if (ENT) r.ent = r.logs - LN2F * (a.t / a.s);
-    return r;
-}
-
-template <typename T, int G, int NT, bool ENT>
-__global__ void __launch_bounds__(NT) k_label_logprobs(const T *logits, long long rows, long long K, long long stride,
-                                                       Idx labels, float inv_t, float *logp, float *lse, float *ent) {
-    __shared__ RowSum scratch[33];
-    pdl_wait();
-    const int tid = threadIdx.x % G;
-    const float c = (float)(LOG2E * inv_t);
-    const long long step = (long long)gridDim.x * (NT / G);
-    for (long long i = (long long)blockIdx.x * (NT / G) + threadIdx.x / G; i < rows; i += step) {
-        const long long y = labels.at(i);
-        if (y < 0) {
-            if (tid == 0) {
-                logp[i] = 0.0f;
-                lse[i] = 0.0f;
-                if (ENT) ent[i] = 0.0f;
-            }
-            continue;
-        }
-        const T *row = logits + i * stride;
-        const RowSum a = group_join<G, ENT>(row_scan<T, G, ENT>(row, K, tid, c), c, scratch);
-        if (tid == 0) {
-            const RowStat r = row_stat<T, ENT>(a, row, K, y, inv_t);
-            logp[i] = r.logp;
-            lse[i] = r.lse;
-            if (ENT) ent[i] = r.ent;
-        }
-    }
-}
-
-// One row of gradient: d x_j = g ([j = y] - p_j) - ge p_j (log p_j + H), with
-// log2 p_j = (x_j - top) c - b (subtracting a top near the row's maximum first
-// keeps the digits of rows whose logits are all huge); `empty` rows get zeros.
-struct RowGrad {
-    float top, c, b, g, ge, ent;
-    int empty;
-};
-__device__ __forceinline__ float grad_at(const RowGrad &r, float x) {
-    const float d = fmaf(x - r.top, r.c, -r.b);
-    const float p = exp2_fast(d);
-    const float h = fmaf(fmaxf(d, D_FLOOR), LN2F, r.ent);
-    return -p * fmaf(r.ge, h, r.g);
-}
-
-template <typename T, int G>
-__device__ __forceinline__ void row_grad(const T *row, T *out, long long K, long long y, int tid, const RowGrad &r) {
-    constexpr int N = Vec<T>::N;
-    auto single = [&](long long j) {
-        float v = r.empty ? 0.0f : grad_at(r, Vec<T>::to(row[j]));
-        if (j == y && !r.empty) v += r.g;
-        out[j] = Vec<T>::from(v);
-    };
-    const RowCut cut = row_cut(row, K);
-    const bool vec = G > 32 && (reinterpret_cast<uintptr_t>(row) - reinterpret_cast<uintptr_t>(out)) % 16 == 0;
-    if (!vec) {  // a warp's row, or an output that is aligned otherwise than its input
-        for (long long j = tid; j < K; j += G) single(j);
-        return;
-    }
-    if (tid < cut.head) single(tid);
-    const uint4 *v = reinterpret_cast<const uint4 *>(row + cut.head);
-    uint4 *o = reinterpret_cast<uint4 *>(out + cut.head);
-    for (long long i = tid; i < cut.vecs; i += G) {
-        float f[N];
-        Vec<T>::unpack(v[i], f);
-        const long long j0 = cut.head + i * N;
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            f[k] = r.empty ? 0.0f : grad_at(r, f[k]);
-            if (j0 + k == y && !r.empty) f[k] += r.g;
-        }
-        o[i] = Vec<T>::pack(f);
-    }
-    for (long long j = cut.head + cut.vecs * N + tid; j < K; j += G) single(j);
-}
-
-// Beyond this |lse| its rounding alone moves every p by more than 2^-16, and
-// the row is summed again.
-constexpr float LSE_EXACT = 256.0f;
-
-template <typename T, int G, int NT>
-__global__ void __launch_bounds__(NT) k_label_logprobs_grad(const T *logits, long long rows, long long K,
-                                                            long long stride, Idx labels, float temperature,
-                                                            const float *lse, const float *grad_logp, const float *ent,
-                                                            const float *grad_ent, T *out, long long out_stride) {
-    __shared__ RowSum scratch[33];
-    pdl_wait();
-    const int tid = threadIdx.x % G;
-    const float inv_t = 1.0f / temperature;
-    const float c = (float)(LOG2E * inv_t);
-    const long long step = (long long)gridDim.x * (NT / G);
-    for (long long i = (long long)blockIdx.x * (NT / G) + threadIdx.x / G; i < rows; i += step) {
-        const long long y = labels.at(i);
-        RowGrad r;
-        const T *row = logits + i * stride;
-        r.c = c;
-        r.top = lse[i] * temperature;
-        r.b = 0.0f;
-        r.empty = y < 0 || lse[i] == -INFINITY;
-        if (!r.empty && fabsf(lse[i]) > LSE_EXACT) {
-            const RowSum a = group_join<G, false>(row_scan<T, G, false>(row, K, tid, c), c, scratch);
-            r.top = finite_top(a.m);
-            r.b = log2f(a.s);
-        }
-        r.g = y < K ? grad_logp[i] * inv_t : NAN;
-        r.ge = grad_ent ? grad_ent[i] * inv_t : 0.0f;
-        r.ent = grad_ent ? ent[i] : 0.0f;
-        row_grad<T, G>(row, out + i * out_stride, K, y, tid, r);
-    }
-}
 
 // ------------------------------------------------------- exact totals --
 // A sum of real numbers as a 128-bit two's complement number of 2^-64ths, so
@@ -669,10 +343,12 @@ struct PolicyCount {
     const Acc *acc;
     const int *ids;                   // sequence of each row (rows of logits), else null
 };
-__device__ __forceinline__ double token_weight(const PolicyRule &r, const PolicyCount &n, long long q) {
-    if (!r.by_sequence) return n.total[0] ? 1.0 / (double)n.total[0] : 0.0;
-    if (q < 0) return 0.0;
-    return 1.0 / ((double)acc_count(n.acc[q]) * (double)n.total[1]);
+// In fp32: one rounding of a count and one of the quotient.
+__device__ __forceinline__ float token_weight(const PolicyCount &n) {
+    return n.total[0] ? 1.0f / (float)n.total[0] : 0.0f;
+}
+__device__ __forceinline__ float seq_weight(const PolicyCount &n, long long q) {
+    return 1.0f / ((float)acc_count(n.acc[q]) * (float)n.total[1]);
 }
 
 constexpr int POL_STATS = 4;  // policy term, kl, entropy, clipped
@@ -731,6 +407,7 @@ __global__ void __launch_bounds__(TOK_THREADS) k_policy_tokens(const float *logp
     __shared__ double scratch[33];
     pdl_wait();
     double sum[POL_STATS] = {};
+    const float w_all = rule.by_sequence ? 0.0f : token_weight(cnt);
     for (long long t0 = (long long)blockIdx.x * TOK_TILE; t0 < T; t0 += (long long)gridDim.x * TOK_TILE) {
         const long long t1 = t0 + TOK_TILE < T ? t0 + TOK_TILE : T;
         if (off.p) tile_span(off, S, t0, t1, span);
@@ -741,68 +418,19 @@ __global__ void __launch_bounds__(TOK_THREADS) k_policy_tokens(const float *logp
             const long long q = off.p ? token_seq(off, S, span[0], span[1], t) : -1;
             float g = 0.0f;
             if ((!mask || mask[t]) && (q >= 0 || !(rule.by_sequence || rule.adv_by_sequence))) {
-                const double w = token_weight(rule, cnt, q);
+                const float w = rule.by_sequence ? seq_weight(cnt, q) : w_all;
                 const PolicyTerm p = policy_term(rule, logp[t], old[t], adv[rule.adv_by_sequence ? q : t],
                                                  rule.kl_kind ? ref[t] : 0.0f);
-                g = (float)w * (rule.kl_coef != 0.0f ? fmaf(rule.kl_coef, p.dkl, p.dpg) : p.dpg);
-                sum[0] += w * p.pg;
-                sum[1] += w * p.kl;
-                sum[3] += w * p.cut;
+                g = w * (rule.kl_coef != 0.0f ? fmaf(rule.kl_coef, p.dkl, p.dpg) : p.dpg);
+                sum[0] += (double)w * p.pg;
+                sum[1] += (double)w * p.kl;
+                sum[3] += (double)w * p.cut;
             }
             grad[t] = g;
         }
         __syncthreads();
     }
     policy_partial(sum, scratch, partial);
-}
-
-// Per-row policy step: sums of the row, the loss's terms, the row's gradient.
-template <typename T, int G, int NT>
-__global__ void __launch_bounds__(NT) k_policy_rows(const T *logits, long long rows, long long K, long long stride,
-                                                    Idx labels, float inv_t, const float *old, const float *adv,
-                                                    const float *ref, const uint8_t *mask, PolicyRule rule,
-                                                    PolicyCount cnt, float *logp, T *out, long long out_stride,
-                                                    double *partial) {
-    __shared__ RowSum scratch[33];
-    __shared__ double dscratch[33];
-    pdl_wait();
-    const int tid = threadIdx.x % G;
-    const float c = (float)(LOG2E * inv_t);
-    const long long step = (long long)gridDim.x * (NT / G);
-    double sum[POL_STATS] = {};
-    for (long long i = (long long)blockIdx.x * (NT / G) + threadIdx.x / G; i < rows; i += step) {
-        const long long y = labels.at(i);
-        const long long q = cnt.ids ? cnt.ids[i] : -1;
-        const T *row = logits + i * stride;
-        RowGrad r{0.0f, c, 0.0f, 0.0f, 0.0f, 0.0f, 1};
-        float lp = 0.0f;
-        if (y >= 0 && (!mask || mask[i]) && (q >= 0 || !(rule.by_sequence || rule.adv_by_sequence))) {
-            const RowSum a = group_join<G, true>(row_scan<T, G, true>(row, K, tid, c), c, scratch);
-            const RowStat st = row_stat<T, true>(a, row, K, y, inv_t);
-            lp = st.logp;
-            const double w = token_weight(rule, cnt, q);
-            const PolicyTerm p = policy_term(rule, lp, old[i], adv[rule.adv_by_sequence ? q : i],
-                                             rule.kl_kind ? ref[i] : 0.0f);
-            const float wg = (float)(w * rule.grad_scale) * inv_t;
-            r.g = wg * (rule.kl_coef != 0.0f ? fmaf(rule.kl_coef, p.dkl, p.dpg) : p.dpg);
-            r.ge = -wg * rule.ent_coef;
-            r.ent = st.ent;
-            r.top = finite_top(a.m);
-            r.b = log2f(a.s);
-            r.empty = a.s == 0.0f;
-            if (tid == 0) {
-                sum[0] += w * p.pg;
-                sum[1] += w * p.kl;
-                sum[2] += w * st.ent;
-                sum[3] += w * p.cut;
-            }
-        }
-        if (G > 32) __syncthreads();  // in place: the label's logit is read before it is overwritten
-        else __syncwarp();
-        if (tid == 0) logp[i] = lp;
-        row_grad<T, G>(row, out + i * out_stride, K, y, tid, r);
-    }
-    policy_partial(sum, dscratch, partial);
 }
 
 // stats: loss, policy term, kl, entropy, share clipped (weighted means)
@@ -844,90 +472,15 @@ static int check_index(const char *name, int bytes) {
     WGB_CHECK_ARG(bytes == 4 || bytes == 8, "%s must be 4- or 8-byte integers", name);
     return WGB_OK;
 }
-static int check_logits(const void *logits, int dtype, long long rows, long long K, long long stride, float temperature) {
-    WGB_CHECK_ARG(dtype >= 0 && dtype <= 2, "logits dtype must be 0 (float32), 1 (bfloat16) or 2 (float16)");
-    WGB_CHECK_ARG(rows >= 0 && K >= 1, "logits need at least one class");
-    WGB_CHECK_ARG(rows <= 1 || stride >= K, "rows of logits overlap: stride %lld, %lld classes", stride, K);
-    WGB_CHECK_ARG(temperature > 0.0f && !isinf(temperature), "temperature must be positive and finite");
-    WGB_CHECK_ARG(rows == 0 || logits != nullptr, "logits is null");
-    const int size = dtype == 0 ? 4 : 2;
-    WGB_CHECK_ARG(reinterpret_cast<uintptr_t>(logits) % size == 0, "logits are not aligned to their type");
-    return WGB_OK;
-}
 #define WGB_TRY(...)                      \
     do {                                  \
         const int rc_ = (__VA_ARGS__);    \
         if (rc_ != WGB_OK) return rc_;    \
     } while (0)
 
-// Rows up to this many classes take a warp each, longer ones a block.
-constexpr long long WARP_ROW = 1024;
-constexpr int ROW_THREADS = 512;
-
-template <typename F>
-static int by_dtype(int dtype, F f) {
-    return dtype == 0 ? f((float *)nullptr) : dtype == 1 ? f((__nv_bfloat16 *)nullptr) : f((__half *)nullptr);
-}
-
 }  // namespace wgb
 
 using namespace wgb;
-
-extern "C" int wgb_label_logprobs(const void *logits, int32_t dtype, int64_t rows, int64_t classes, int64_t row_stride,
-                                  const void *labels, int32_t label_bytes, float temperature, float *logp, float *lse,
-                                  float *entropy, void *stream) {
-    WGB_TRY(check_logits(logits, dtype, rows, classes, row_stride, temperature));
-    WGB_TRY(check_index("labels", label_bytes));
-    if (rows == 0) return WGB_OK;
-    WGB_CHECK_ARG(labels && logp && lse, "labels, logp and lse must not be null");
-    cudaStream_t st = as_stream(stream);
-    const Idx lab{labels, label_bytes == 8};
-    const float inv_t = 1.0f / temperature;
-    return by_dtype(dtype, [&](auto *tag) -> int {
-        using T = std::remove_pointer_t<decltype(tag)>;
-        const T *x = static_cast<const T *>(logits);
-        auto go = [&](auto ent) -> int {
-            constexpr bool ENT = decltype(ent)::value;
-            if (classes <= WARP_ROW)
-                WGB_PDL("k_label_logprobs", k_label_logprobs<T, 32, 256, ENT>, dim3(grid_of(rows, 8, sm_count() * 8)),
-                        dim3(256), 0, st, x, rows, classes, row_stride, lab, inv_t, logp, lse, entropy);
-            else
-                WGB_PDL("k_label_logprobs", k_label_logprobs<T, ROW_THREADS, ROW_THREADS, ENT>,
-                        dim3(grid_of(rows, 1, sm_count() * 4)), dim3(ROW_THREADS), 0, st, x, rows, classes, row_stride,
-                        lab, inv_t, logp, lse, entropy);
-            return WGB_OK;
-        };
-        return entropy ? go(std::true_type{}) : go(std::false_type{});
-    });
-}
-
-extern "C" int wgb_label_logprobs_grad(const void *logits, int32_t dtype, int64_t rows, int64_t classes,
-                                       int64_t row_stride, const void *labels, int32_t label_bytes, float temperature,
-                                       const float *lse, const float *grad_logp, const float *entropy,
-                                       const float *grad_entropy, void *grad, int64_t grad_stride, void *stream) {
-    WGB_TRY(check_logits(logits, dtype, rows, classes, row_stride, temperature));
-    WGB_TRY(check_logits(grad, dtype, rows, classes, grad_stride, temperature));
-    WGB_TRY(check_index("labels", label_bytes));
-    if (rows == 0) return WGB_OK;
-    WGB_CHECK_ARG(labels && lse && grad_logp, "labels, lse and grad_logp must not be null");
-    WGB_CHECK_ARG(!grad_entropy || entropy, "grad_entropy needs the entropies");
-    cudaStream_t st = as_stream(stream);
-    const Idx lab{labels, label_bytes == 8};
-    return by_dtype(dtype, [&](auto *tag) -> int {
-        using T = std::remove_pointer_t<decltype(tag)>;
-        const T *x = static_cast<const T *>(logits);
-        T *o = static_cast<T *>(grad);
-        if (classes <= WARP_ROW)
-            WGB_PDL("k_label_logprobs_grad", k_label_logprobs_grad<T, 32, 256>, dim3(grid_of(rows, 8, sm_count() * 8)),
-                    dim3(256), 0, st, x, rows, classes, row_stride, lab, temperature, lse, grad_logp, entropy,
-                    grad_entropy, o, grad_stride);
-        else
-            WGB_PDL("k_label_logprobs_grad", k_label_logprobs_grad<T, ROW_THREADS, ROW_THREADS>,
-                    dim3(grid_of(rows, 1, sm_count() * 4)), dim3(ROW_THREADS), 0, st, x, rows, classes, row_stride, lab,
-                    temperature, lse, grad_logp, entropy, grad_entropy, o, grad_stride);
-        return WGB_OK;
-    });
-}
 
 extern "C" int64_t wgb_preference_ws_bytes(int64_t sequences, int32_t ragged) {
     if (sequences < 0) return 0;
@@ -977,7 +530,7 @@ extern "C" int wgb_preference_loss(const float *logp, const float *ref_logp, int
 }
 
 namespace wgb {
-constexpr int POL_BLOCKS_PER_SM = 8;
+constexpr int POL_BLOCKS_PER_SM = 16;
 struct PolicyWs {
     unsigned long long *total;
     double *partial;
@@ -1069,54 +622,3 @@ extern "C" int wgb_policy_loss(const float *logp, const float *old_logp, const f
     return WGB_OK;
 }
 
-extern "C" int wgb_policy_loss_logits(const void *logits, int32_t dtype, int64_t rows, int64_t classes,
-                                      int64_t row_stride, const void *labels, int32_t label_bytes, float temperature,
-                                      const float *old_logp, const float *advantages, const float *ref_logp,
-                                      const uint8_t *mask, const void *offsets, int32_t offset_bytes, int64_t sequences,
-                                      int32_t adv_by_sequence, int32_t by_sequence, float clip_low, float clip_high,
-                                      int32_t kl_kind, float kl_coef, float entropy_coef, float grad_scale, void *ws,
-                                      int64_t ws_bytes, float *stats, float *logp, void *grad, int64_t grad_stride,
-                                      void *stream) {
-    WGB_TRY(check_logits(logits, dtype, rows, classes, row_stride, temperature));
-    WGB_TRY(check_logits(grad, dtype, rows, classes, grad_stride, temperature));
-    WGB_TRY(check_index("labels", label_bytes));
-    WGB_CHECK_ARG(sequences >= 0 && sequences < (1ll << 31), "too many sequences");
-    PolicyRule rule;
-    WGB_TRY(policy_rule(
-        PolicyArgs{clip_low, clip_high, kl_coef, entropy_coef, grad_scale, kl_kind, by_sequence, adv_by_sequence},
-        ref_logp, rows, rule));
-    if (offsets) WGB_TRY(check_index("offsets", offset_bytes));
-    WGB_CHECK_ARG(offsets || (!by_sequence && !adv_by_sequence), "a mean or advantages by sequence need offsets");
-    WGB_CHECK_ARG(rows == 0 || (labels && old_logp && advantages && logp),
-                  "labels, old_logp, advantages and logp must not be null");
-    WGB_CHECK_ARG(stats != nullptr, "stats must not be null");
-    const bool seqs = by_sequence || adv_by_sequence;
-    WGB_CHECK_ARG(ws && ws_bytes >= wgb_policy_ws_bytes(rows, sequences, 1), "workspace too small");
-    WGB_CHECK_ARG(reinterpret_cast<uintptr_t>(ws) % 16 == 0, "workspace is not aligned to 16 bytes");
-    cudaStream_t st = as_stream(stream);
-    const PolicyWs w = policy_ws(ws, rows, sequences, seqs);
-    const Idx off{seqs ? offsets : nullptr, offset_bytes == 8}, lab{labels, label_bytes == 8};
-    WGB_TRY(policy_counts(w, mask, lab, rows, off, sequences, rule, st));
-    const PolicyCount cnt{w.total, w.acc, w.ids};
-    const float inv_t = 1.0f / temperature;
-    int grid = 1;
-    WGB_TRY(by_dtype(dtype, [&](auto *tag) -> int {
-        using T = std::remove_pointer_t<decltype(tag)>;
-        const T *x = static_cast<const T *>(logits);
-        T *o = static_cast<T *>(grad);
-        if (classes <= WARP_ROW) {
-            grid = grid_of(rows, 8, sm_count() * POL_BLOCKS_PER_SM);
-            WGB_PDL("k_policy_rows", k_policy_rows<T, 32, 256>, dim3(grid), dim3(256), 0, st, x, rows, classes,
-                    row_stride, lab, inv_t, old_logp, advantages, ref_logp, mask, rule, cnt, logp, o, grad_stride,
-                    w.partial);
-        } else {
-            grid = grid_of(rows, 1, sm_count() * 4);
-            WGB_PDL("k_policy_rows", k_policy_rows<T, ROW_THREADS, ROW_THREADS>, dim3(grid), dim3(ROW_THREADS), 0, st,
-                    x, rows, classes, row_stride, lab, inv_t, old_logp, advantages, ref_logp, mask, rule, cnt, logp, o,
-                    grad_stride, w.partial);
-        }
-        return WGB_OK;
-    }));
-    WGB_PDL("k_policy_finish", k_policy_finish, dim3(1), dim3(256), 0, st, (const double *)w.partial, grid, rule, stats);
-    return WGB_OK;
-}

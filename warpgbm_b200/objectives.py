@@ -116,10 +116,17 @@ def _logits(t, name="logits"):
 
 
 def _grad_like(logits, stride, out):
-    """The gradient's buffer and row stride: a new one, or the caller's."""
+    """The gradient's buffer and row stride: the caller's, or a new one whose
+    rows lie on 16-byte boundaries as the logits' do (the kernels then move
+    whole words), which leaves a few elements between rows where theirs do."""
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        return out, logits.shape[1]
+        n, k = logits.shape
+        size = logits.element_size()
+        out_stride, off = k + (stride - k) % (16 // size), logits.data_ptr() % 16 // size
+        if out_stride == k and off == 0:
+            return torch.empty((n, k), dtype=logits.dtype, device=logits.device), k
+        buf = torch.empty(n * out_stride + off, dtype=logits.dtype, device=logits.device)
+        return buf.as_strided((n, k), (out_stride, 1), off), out_stride
     n, k, out_stride = _logits(out, "out")
     if out.dtype != logits.dtype or out.shape != logits.shape or out.device != logits.device:
         raise ValueError("out must have the dtype, shape and device of logits")
@@ -190,7 +197,8 @@ def label_logprobs_grad(logits, labels, lse, grad_logp, *, temperature=1.0, entr
                         out=None) -> torch.Tensor:
     """Gradient to the logits from the gradients to ``logp`` (and, with
     ``entropy`` as label_logprobs gave it, to the entropy).  ``out`` may be the
-    logits themselves."""
+    logits themselves; without it rows of odd length may lie apart as theirs do
+    (their stride is that of the logits up to multiples of 16 bytes)."""
     n, k, stride = _logits(logits)
     dev = logits.device
     y = _vector(labels, "labels", n, _INTS, dev)
