@@ -539,6 +539,7 @@ struct RowsArgs {
     PolicyRule rule;
     PolicyCount cnt;
     double *partial;
+    float *stats;
 };
 
 // Beyond this |lse| its rounding alone moves every p by more than 2^-16, and
@@ -748,9 +749,8 @@ __global__ void __launch_bounds__(NT, GL > 32 ? 1024 / NT : 4) k_rows(const __gr
         }
     }
     if (OP == ROW_POLICY) {
-        if (!BLOCK) policy_partial(own_tot, dscratch, a.partial);
-        else if (threadIdx.x == 0)
-            for (int k = 0; k < POL_STATS; ++k) a.partial[(long long)blockIdx.x * POL_STATS + k] = shared_tot[k];
+        if (!BLOCK) policy_end_block(own_tot, a.rule, a.cnt.ticket, a.partial, a.stats, dscratch);
+        else if (threadIdx.x < 32) policy_end(shared_tot, a.rule, a.cnt.ticket, a.partial, a.stats);
     }
 }
 
@@ -819,8 +819,7 @@ __global__ void __launch_bounds__(NT, 2) k_rows_long(const __grid_constant__ Row
             }
         }
     }
-    if (OP == ROW_POLICY && tid == 0)
-        for (int k = 0; k < POL_STATS; ++k) a.partial[(long long)blockIdx.x * POL_STATS + k] = tot[k];
+    if (OP == ROW_POLICY && tid < 32) policy_end(tot, a.rule, a.cnt.ticket, a.partial, a.stats);
 }
 
 // ------------------------------------------------------ ring of copies --
@@ -1028,8 +1027,7 @@ __global__ void __launch_bounds__(RING_NT, ring_blocks<OP>()) k_rows_ring(const 
                 }
             }
         }
-        if (OP == ROW_POLICY && lane == 0)
-            for (int j = 0; j < POL_STATS; ++j) a.partial[(long long)blockIdx.x * POL_STATS + j] = tot[j];
+        if (OP == ROW_POLICY) policy_end(tot, a.rule, a.cnt.ticket, a.partial, a.stats);
     } else {  // ------------------------------------------- sums and gradients
         int slot = 0;
         unsigned parity = 0;
@@ -1217,7 +1215,7 @@ __global__ void __launch_bounds__(TILE_ROWS) k_rows_tile(const __grid_constant__
         }
         __syncthreads();
     }
-    if (OP == ROW_POLICY) policy_partial(tot, dscratch, a.partial);
+    if (OP == ROW_POLICY) policy_end_block(tot, a.rule, a.cnt.ticket, a.partial, a.stats, dscratch);
 }
 
 // ---------------------------------------------------------------- host --
@@ -1231,34 +1229,6 @@ static int check_logits(const void *logits, int dtype, long long rows, long long
     const int size = dtype == 0 ? 4 : 2;
     WGB_CHECK_ARG(reinterpret_cast<uintptr_t>(logits) % size == 0, "logits are not aligned to their type");
     return WGB_OK;
-}
-
-// Resident clusters (or blocks) of a kernel on the current device.
-template <typename K>
-static int resident(K kernel, int nt, int cl, int smem, int (&cache)[64]) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sm_count();
-    if (!cache[dev]) {
-        int n = 0;
-        if (cl == 1) {
-            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, nt, smem) != cudaSuccess) n = 0;
-            n *= sm_count();
-        } else {
-            cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(cl);
-            cfg.blockDim = dim3(nt);
-            cfg.dynamicSmemBytes = smem;
-            cudaLaunchAttribute at[1];
-            at[0].id = cudaLaunchAttributeClusterDimension;
-            at[0].val.clusterDim.x = cl;
-            at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-            cfg.attrs = at;
-            cfg.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
-        }
-        cache[dev] = n > 0 ? n : 1;
-    }
-    return cache[dev];
 }
 
 // Launches `kernel` over `units` rows (or tiles): one wave of persistent blocks.
@@ -1432,7 +1402,10 @@ extern "C" int wgb_policy_loss_logits(const void *logits, int32_t dtype, int64_t
     cudaStream_t st = as_stream(stream);
     const PolicyWs w = policy_ws(ws, rows, sequences, seqs);
     const Idx off{seqs ? offsets : nullptr, offset_bytes == 8}, lab{labels, label_bytes == 8};
-    WGB_TRY(policy_counts(w, mask, lab, rows, off, sequences, rule, st));
+    const CountArgs n = count_args(w, mask, lab, rows, off, sequences, rule);
+    static int cache[64];
+    WGB_TRY(launch_all("k_policy_count", k_policy_count<true, GRID_THREADS>, k_policy_count<false, BLOCK_THREADS>,
+                       rows + (by_sequence ? sequences : 0), cache, n, st));
     RowsArgs a = {};
     a.logits = logits;
     a.grad = grad;
@@ -1448,10 +1421,11 @@ extern "C" int wgb_policy_loss_logits(const void *logits, int32_t dtype, int64_t
     a.ref = ref_logp;
     a.mask = mask;
     a.rule = rule;
-    a.cnt = PolicyCount{w.total, w.acc, w.ids};
+    a.cnt = w.cnt;
     a.partial = w.partial;
+    a.stats = stats;
     int grid = 0;
-    if (rows) WGB_TRY(run_typed<ROW_POLICY>(dtype, true, a, grid, st));
-    WGB_PDL("k_policy_finish", k_policy_finish, dim3(1), dim3(256), 0, st, (const double *)w.partial, grid, rule, stats);
+    if (rows) return run_typed<ROW_POLICY>(dtype, true, a, grid, st);
+    WGB_CUDA(cudaMemsetAsync(stats, 0, 5 * sizeof(float), st));
     return WGB_OK;
 }

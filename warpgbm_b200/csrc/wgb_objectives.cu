@@ -3,10 +3,18 @@
 // include/warpgbm_b200.h; the calls that take rows of logits are in
 // wgb_logits.cu).
 //
+// A call is one launch.  What comes first has to be complete before the next
+// part can start (kept tokens are counted before their gradient is scaled, a
+// sequence is summed before its pairs are compared), so the parts are separated
+// by a barrier: of a cooperative grid, or of the one block that small calls
+// take, which then costs a launch and a few microseconds.
+//
 // Sums over the tokens of a sequence and over the pairs of a sequence are
 // exact: a partial sum formed in a fixed order is added to a 128-bit
-// fixed-point number with integer atomics (Acc), so no result depends on the
+// fixed-point number with integer atomics (Sums), so no result depends on the
 // order of the atomics.
+#include <cooperative_groups.h>
+
 #include <type_traits>
 
 namespace wgb {
@@ -20,62 +28,135 @@ struct Idx {
     }
 };
 
+// Everything before is done, and visible, for the whole launch.
+template <bool GRID>
+__device__ __forceinline__ void all_sync() {
+    if constexpr (GRID) cooperative_groups::this_grid().sync();
+    else __syncthreads();
+}
+
+__device__ __forceinline__ double block_sum(double v, double *scratch /* >= 33 */) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    v = warp_sum(v);
+    if (lane == 0) scratch[w] = v;
+    __syncthreads();
+    if (w == 0) {
+        v = warp_sum(lane < nw ? scratch[lane] : 0.0);
+        if (lane == 0) scratch[32] = v;
+    }
+    __syncthreads();
+    v = scratch[32];
+    __syncthreads();
+    return v;
+}
+
+// The block's thread 0 has written the block's share of what `ticket` counts;
+// whether this block is the last to have.  One warp calls it.
+__device__ __forceinline__ bool last_of_grid(unsigned *ticket) {
+    unsigned mine = 0;
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+        __threadfence();
+        mine = atomicAdd(ticket, 1u);
+        __threadfence();
+    }
+    return __shfl_sync(0xffffffffu, mine, 0) == gridDim.x - 1;
+}
+
 // ------------------------------------------------------- exact totals --
-// A sum of real numbers as a 128-bit two's complement number of 2^-64ths, so
-// that adding is associative.  A term is cut to a multiple of 2^-64; a term of
-// 2^40 or more counts as infinite, and infinities and NaN are kept apart.
-struct Acc {
-    unsigned long long lo;
-    long long hi;
-    unsigned long long n;  // terms counted (tokens kept); the top bits hold what is not finite
+// Sums of real numbers as 128-bit two's complement numbers of 2^-64ths, so that
+// adding is associative.  A term is cut to a multiple of 2^-64; a term of 2^40
+// or more counts as infinite, and infinities and NaN are kept in a byte apart.
+// All of it starts as zeros.
+struct Sums {
+    unsigned long long *lo_hi;  // [n][2]
+    unsigned *odd;              // a byte each: 1 +inf, 2 -inf, 4 NaN
+    __device__ __forceinline__ void add(long long i, double v) const {
+        const double u = fabs(v);
+        if (!(u < 1099511627776.0)) {
+            atomicOr(odd + (i >> 2), (u != u ? 4u : v > 0 ? 1u : 2u) << (8 * (i & 3)));
+            return;
+        }
+        const double whole = floor(u);
+        unsigned long long lo = (unsigned long long)((u - whole) * 18446744073709551616.0);
+        long long hi = (long long)whole;
+        if (v < 0) {
+            hi = ~hi + (lo == 0);
+            lo = ~lo + 1ull;
+        }
+        if (lo) {
+            const unsigned long long old = atomicAdd(lo_hi + 2 * i, lo);
+            hi += old + lo < old;  // carry
+        }
+        if (hi) atomicAdd(lo_hi + 2 * i + 1, (unsigned long long)hi);
+    }
+    __device__ __forceinline__ double value(long long i) const {
+        const unsigned o = odd[i >> 2] >> (8 * (i & 3)) & 7u;
+        const ulonglong2 p = reinterpret_cast<const ulonglong2 *>(lo_hi)[i];
+        if (o) return o == 1 ? INFINITY : o == 2 ? -INFINITY : NAN;
+        unsigned long long lo = p.x;
+        long long hi = (long long)p.y;
+        const bool neg = hi < 0;
+        if (neg) {
+            hi = ~hi + (lo == 0);
+            lo = ~lo + 1ull;
+        }
+        const double v = (double)hi + (double)lo * 5.42101086242752217e-20;
+        return neg ? -v : v;
+    }
 };
-constexpr int ACC_ODD = 61;  // +inf, -inf, NaN in bits 61 to 63 of n
-__device__ __forceinline__ unsigned long long acc_count(const Acc &a) { return a.n & ((1ull << ACC_ODD) - 1ull); }
-
-__device__ __forceinline__ void acc_add(Acc *a, double v) {
-    const double u = fabs(v);
-    if (!(u < 1099511627776.0)) {
-        atomicOr(&a->n, (u != u ? 4ull : v > 0 ? 1ull : 2ull) << ACC_ODD);
-        return;
+// The same memory for terms of at most `bound` in magnitude, n of them at most:
+// one addition to one of two 64-bit numbers, each a multiple of a power of two.
+// Terms from 2^-17 bound on count in units of bound 2^-62 n (2^-25 of the term or
+// less), smaller ones in units 2^17 times finer.
+struct GridSums {
+    Sums s;
+    double unit, inv, small;  // 1 / unit of the first number, the unit; below `small`: the second
+    __device__ __forceinline__ GridSums(const Sums &of, float bound, long long n) : s(of) {
+        int e = 0, m = 0;
+        bound = fminf(bound, 3.4028234e38f);
+        frexpf(bound, &e);             // bound <= 2^e
+        frexp((double)n, &m);          // n < 2^m
+        const int k = 62 - m - e;
+        unit = ldexp(1.0, k);
+        inv = ldexp(1.0, -k);
+        small = ldexp((double)bound, -17);
     }
-    const double whole = floor(u);
-    unsigned long long lo = (unsigned long long)((u - whole) * 18446744073709551616.0);
-    long long hi = (long long)whole;
-    if (v < 0) {
-        hi = ~hi + (lo == 0);
-        lo = ~lo + 1ull;
+    __device__ __forceinline__ void add(long long i, float v) const {
+        const double u = fabs((double)v);
+        if (!(u < 1e300)) {
+            atomicOr(s.odd + (i >> 2), (u != u ? 4u : v > 0 ? 1u : 2u) << (8 * (i & 3)));
+            return;
+        }
+        const bool fine = u < small;
+        const long long n = __double2ll_rn((double)v * (fine ? unit * 131072.0 : unit));
+        if (n) atomicAdd(s.lo_hi + 2 * i + fine, (unsigned long long)n);
     }
-    if (lo) {
-        const unsigned long long old = atomicAdd(&a->lo, lo);
-        hi += old + lo < old;  // carry
+    __device__ __forceinline__ double value(long long i) const {
+        const unsigned o = s.odd[i >> 2] >> (8 * (i & 3)) & 7u;
+        const ulonglong2 p = reinterpret_cast<const ulonglong2 *>(s.lo_hi)[i];
+        if (o) return o == 1 ? INFINITY : o == 2 ? -INFINITY : NAN;
+        return ((double)(long long)p.x + (double)(long long)p.y * (1.0 / 131072.0)) * inv;
     }
-    if (hi) atomicAdd(reinterpret_cast<unsigned long long *>(&a->hi), (unsigned long long)hi);
+};
+__host__ __device__ constexpr long long sums_bytes(long long n) { return 16 * n + (n + 15) / 16 * 16; }
+inline Sums sums_at(char *p, long long n) {
+    return Sums{reinterpret_cast<unsigned long long *>(p), reinterpret_cast<unsigned *>(p + 16 * n)};
 }
 
-__device__ __forceinline__ double acc_value(const Acc &a) {
-    if (const unsigned odd = (unsigned)(a.n >> ACC_ODD)) return odd == 1 ? INFINITY : odd == 2 ? -INFINITY : NAN;
-    unsigned long long lo = a.lo;
-    long long hi = a.hi;
-    const bool neg = hi < 0;
-    if (neg) {
-        hi = ~hi + (lo == 0);
-        lo = ~lo + 1ull;
-    }
-    const double v = (double)hi + (double)lo * 5.42101086242752217e-20;
-    return neg ? -v : v;
-}
-
-__global__ void k_acc_zero(Acc *a, long long n, unsigned long long *extra, int n_extra) {
-    pdl_wait();
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i < n) a[i] = Acc{0ull, 0ll, 0ull};
-    if (i < n_extra) extra[i] = 0ull;
+// Zeroes `bytes` (a multiple of 16) at p, by the whole launch.
+__device__ __forceinline__ void zero_words(void *p, long long bytes) {
+    uint4 *w = static_cast<uint4 *>(p);
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < bytes / 16; i += (long long)gridDim.x * blockDim.x)
+        w[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
 // ----------------------------------------------------------- sequences --
-constexpr int TOK_THREADS = 256;
-constexpr int TOK_EACH = 4;
-constexpr int TOK_TILE = TOK_THREADS * TOK_EACH;
+// The tokens are cut into one range for each warp, and a warp goes through its
+// range in steps of STEP tokens, four neighbouring ones to a lane (one 16-byte
+// access to each array), keeping the sequence that it is in: only the start of a
+// range is searched for.
+constexpr int STEP = 128;
 
 // First i in [lo, hi) with off[i] > t, else hi; every lane of a warp calls it.
 __device__ __forceinline__ long long upper_bound_warp(const Idx &off, long long lo, long long hi, long long t) {
@@ -100,24 +181,98 @@ __device__ __forceinline__ long long upper_bound_one(const Idx &off, long long l
     return lo;
 }
 
-// The sequences that a tile of tokens [t0, t1) can meet: q0 .. q1.
-__device__ __forceinline__ void tile_span(const Idx &off, long long S, long long t0, long long t1, long long *span) {
-    const int w = threadIdx.x >> 5;
-    if (w < 2) {
-        const long long u = upper_bound_warp(off, 0, S + 1, w == 0 ? t0 : t1 - 1) - 1;
-        if ((threadIdx.x & 31) == 0) span[w] = u;
-    }
-    __syncthreads();
-}
-// Sequence of token t of a tile whose span is q0 .. q1, or -1 where none holds it.
-__device__ __forceinline__ long long token_seq(const Idx &off, long long S, long long q0, long long q1, long long t) {
-    const long long q = upper_bound_one(off, q0 + 1, q1 + 1, t) - 1;
-    return q < S ? q : -1;
+// The warp's place among the launch's warps, and its range of tokens.
+__device__ __forceinline__ long long warp_index() { return ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; }
+__device__ __forceinline__ long long warp_count() { return ((long long)gridDim.x * blockDim.x) >> 5; }
+struct Range {
+    long long a, b;
+};
+__device__ __forceinline__ Range warp_range(long long T) {
+    const long long steps = (T + STEP - 1) / STEP, n = warp_count(), i = warp_index();
+    const long long each = steps / n, more = steps % n;
+    const long long first = i * each + (i < more ? i : more);
+    const long long a = first * STEP, b = (first + each + (i < more)) * STEP;
+    return Range{a < T ? a : T, b < T ? b : T};
 }
 
-// Adds v (and counts 1) for the lanes of a warp with keep, by sequence q:
-// neighbouring lanes of one sequence are summed first.
-__device__ __forceinline__ void warp_seq_add(Acc *acc, long long q, double v, int n, bool with_sum) {
+// Where a warp is: sequence q (-1 before the first, S after the last) holds the
+// tokens up to `end`.  All lanes have the same.
+struct Place {
+    long long q, end;
+    __device__ __forceinline__ void find(const Idx &off, long long S, long long lo, long long t) {
+        q = upper_bound_warp(off, lo, S + 1, t) - 1;
+        end = q < S ? off.at(q + 1) : LLONG_MAX;
+    }
+    // To the sequence of token t = end.
+    __device__ __forceinline__ void next(const Idx &off, long long S, long long t) {
+        if (q + 2 <= S && off.at(q + 2) > t) {
+            ++q;
+            end = off.at(q + 1);
+        } else {
+            find(off, S, q + 1 < S + 1 ? q + 1 : S + 1, t);
+        }
+    }
+    __device__ __forceinline__ bool valid(long long S) const { return q >= 0 && q < S; }
+};
+// Whether a step that ends at t1 meets so many sequences that lanes had better
+// look for their own.
+constexpr int MANY = 6;
+__device__ __forceinline__ bool many_seqs(const Idx &off, long long S, const Place &at, long long t1) {
+    return at.end < t1 && at.q + MANY <= S && off.at(at.q + MANY) < t1;
+}
+// Sequences of the four tokens from t on (-1: none), at.q .. last being those of
+// the step.
+__device__ __forceinline__ void quad_seqs(const Idx &off, long long S, long long first, long long last, long long t,
+                                          long long (&q)[4]) {
+    long long i = upper_bound_one(off, first + 1, last + 1, t) - 1;
+    long long end = i < last ? off.at(i + 1) : LLONG_MAX;  // first token that is not of `i`
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (t + j >= end) {
+            i = upper_bound_one(off, i + 1, last + 1, t + j) - 1;
+            end = i < last ? off.at(i + 1) : LLONG_MAX;
+        }
+        q[j] = i < S ? i : -1;
+    }
+}
+
+// Four neighbouring values from t on, those past the end as `none`; `whole`:
+// the array may be read 16 (mask: 4) bytes at a time.
+__device__ __forceinline__ void quad_load(const float *p, long long t, long long T, bool whole, float none, float (&v)[4]) {
+    if (whole && t + 4 <= T) {
+        const float4 u = *reinterpret_cast<const float4 *>(p + t);
+        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = t + j < T ? p[t + j] : none;
+    }
+}
+__device__ __forceinline__ void quad_store(float *p, long long t, long long T, bool whole, const float (&v)[4]) {
+    if (whole && t + 4 <= T) {
+        *reinterpret_cast<float4 *>(p + t) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (t + j < T) p[t + j] = v[j];
+    }
+}
+__device__ __forceinline__ void quad_mask(const uint8_t *p, long long t, long long T, bool whole, bool (&k)[4]) {
+    if (!p) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[j] = t + j < T;
+    } else if (whole && t + 4 <= T) {
+        const uchar4 u = *reinterpret_cast<const uchar4 *>(p + t);
+        k[0] = u.x; k[1] = u.y; k[2] = u.z; k[3] = u.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[j] = t + j < T && p[t + j];
+    }
+}
+
+// Calls add(q, v, n) with the sums of v and n over neighbouring lanes of one
+// sequence q >= 0; every lane of a warp calls it.
+template <typename F>
+__device__ __forceinline__ void warp_by_seq(long long q, double v, int n, F add) {
     const int lane = threadIdx.x & 31;
     const unsigned full = 0xffffffffu;
     const long long prev = __shfl_up_sync(full, q, 1);
@@ -133,41 +288,64 @@ __device__ __forceinline__ void warp_seq_add(Acc *acc, long long q, double v, in
         }
     }
     const bool last = lane == 31 || ((heads >> (lane + 1)) & 1u);
-    if (last && q >= 0 && n) {
-        if (with_sum) acc_add(acc + q, v);
-        atomicAdd(&acc[q].n, (unsigned long long)n);
+    if (last && q >= 0 && n) add(q, v, n);
+}
+
+// Sums of a warp's range by sequence: fetch(t, keep, v) gives the four tokens
+// from t on whether they are kept and their values; add(q, v, n), called by one
+// lane, takes what the range has of sequence q.
+template <typename FETCH, typename ADD>
+__device__ __forceinline__ void range_by_seq(const Idx &off, long long S, const Range &r, FETCH fetch, ADD add) {
+    if (r.a >= r.b) return;
+    const int lane = threadIdx.x & 31;
+    Place at;
+    at.find(off, S, 0, r.a);
+    double sum = 0.0;  // of the sequence that the warp is in
+    int count = 0;
+    auto flush = [&]() {
+        const double v = warp_sum(sum);
+        const int n = warp_sum(count);
+        if (lane == 0 && n && at.valid(S)) add(at.q, v, n);
+        sum = 0.0;
+        count = 0;
+    };
+    for (long long t0 = r.a; t0 < r.b; t0 += STEP) {
+        const long long t1 = t0 + STEP < r.b ? t0 + STEP : r.b, t = t0 + lane * 4;
+        bool keep[4];
+        float v[4];
+        fetch(t, keep, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) keep[j] = keep[j] && t + j < t1;
+        if (many_seqs(off, S, at, t1)) {
+            flush();
+            const long long first = at.q;
+            at.find(off, S, at.q + 1, t1 - 1);
+            long long q[4];
+            quad_seqs(off, S, first, at.q, t, q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) warp_by_seq(q[j], keep[j] ? (double)v[j] : 0.0, keep[j], add);
+            continue;
+        }
+        for (long long from = t0; from < t1;) {
+            if (at.end <= from) {
+                flush();
+                at.next(off, S, from);
+                if (at.end <= from) break;  // offsets that do not rise
+            }
+            const long long to = at.end < t1 ? at.end : t1;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (keep[j] && t + j >= from && t + j < to) {
+                    sum += (double)v[j];
+                    ++count;
+                }
+            from = to;
+        }
     }
+    flush();
 }
 
 // --------------------------------------------------------- preference --
-// Sequence sums of logp - ref over the kept tokens.
-__global__ void __launch_bounds__(TOK_THREADS) k_pref_sums(const float *logp, const float *ref, const uint8_t *mask,
-                                                           long long T, Idx off, long long S, Acc *acc) {
-    __shared__ long long span[2];
-    pdl_wait();
-    for (long long t0 = (long long)blockIdx.x * TOK_TILE; t0 < T; t0 += (long long)gridDim.x * TOK_TILE) {
-        const long long t1 = t0 + TOK_TILE < T ? t0 + TOK_TILE : T;
-        tile_span(off, S, t0, t1, span);
-        const long long q0 = span[0], q1 = span[1];
-#pragma unroll
-        for (int e = 0; e < TOK_EACH; ++e) {
-            const long long t = t0 + e * TOK_THREADS + threadIdx.x;
-            long long q = -1;
-            double v = 0.0;
-            int n = 0;
-            if (t < t1) {
-                q = token_seq(off, S, q0, q1, t);
-                if (!mask || mask[t]) {
-                    v = ref ? (double)(logp[t] - ref[t]) : (double)logp[t];
-                    n = 1;
-                }
-            }
-            warp_seq_add(acc, q, v, n, true);
-        }
-        __syncthreads();
-    }
-}
-
 struct PairRule {
     int kind;  // 0 sigmoid, 1 hinge, 2 square
     float beta, smoothing;
@@ -202,94 +380,191 @@ __device__ __forceinline__ PairTerm pair_term(const PairRule &r, float x) {
     return p;
 }
 
-// Score of sequence q: its sum (or mean) of log ratios; NaN out of range.
-__device__ __forceinline__ double seq_score(const Acc *acc, long long S, long long q, const float *logp,
-                                            const float *ref, int average) {
-    if (q < 0 || q >= S) return NAN;
-    if (!acc) return ref ? (double)(logp[q] - ref[q]) : (double)logp[q];
-    const Acc a = acc[q];
-    const double v = acc_value(a);
-    const unsigned long long n = acc_count(a);
-    return average && n ? v / (double)n : v;
-}
+struct PrefArgs {
+    const float *logp, *ref;
+    long long T;
+    Idx off;  // null: every row is a sequence
+    long long S;
+    const uint8_t *mask;
+    Idx chosen, rejected;
+    long long P;
+    const float *weight;
+    PairRule rule;
+    float *loss, *grad, *chosen_reward, *rejected_reward;
+    double *partial;            // a block's share of the loss
+    float *top;                 // a block's largest |weight|
+    void *zeros;                // what has to start as zeros
+    long long zero_bytes;
+    Sums grads, scores;         // by sequence: gradient, sum of log ratios (ragged)
+    unsigned long long *count;  // kept tokens by sequence (ragged)
+    float *diff;                // logp - ref by row (not ragged, with a reference)
+    bool whole, whole_mask;     // arrays on 16-byte (mask: 4-byte) boundaries
+};
 
-__device__ __forceinline__ double block_sum(double v, double *scratch /* >= 33 */) {
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    v = warp_sum(v);
-    if (lane == 0) scratch[w] = v;
-    __syncthreads();
-    if (w == 0) {
-        v = warp_sum(lane < nw ? scratch[lane] : 0.0);
-        if (lane == 0) scratch[32] = v;
-    }
-    __syncthreads();
-    v = scratch[32];
-    __syncthreads();
+// Score of sequence q: its sum (or mean) of log ratios; NaN out of range.
+__device__ __forceinline__ double seq_score(const PrefArgs &a, long long q) {
+    if (q < 0 || q >= a.S) return NAN;
+    if (!a.off.p) return (double)(a.ref ? a.diff : a.logp)[q];
+    const double v = a.scores.value(q);
+    return a.rule.average && a.count[q] ? v / (double)a.count[q] : v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 
-constexpr int PAIR_THREADS = 256;
-constexpr int PAIR_BLOCKS = 592;  // most blocks, each with one partial loss
+constexpr int PAIR_EACH = 4;  // pairs of a thread under way together: they are gathers, and wait for memory
 
-// acc null: every row is its own sequence and scores come from logp itself.
-__global__ void __launch_bounds__(PAIR_THREADS) k_pref_pairs(const float *logp, const float *ref, const Acc *acc,
-                                                             long long S, Idx chosen, Idx rejected, long long P,
-                                                             const float *weight, PairRule rule, Acc *gacc,
-                                                             float *chosen_reward, float *rejected_reward,
-                                                             double *partial) {
+// Bytes: 13 a token read and 4 written, 16 a pair and the gathers of its
+// scores.  Time goes to the barriers and, with many pairs, to the atomics of
+// their gradients: two a pair, which a bound on their terms allows for (the
+// square loss has none and takes up to four).
+template <bool GRID, int NT>
+__global__ void __launch_bounds__(NT) k_preference(const __grid_constant__ PrefArgs a) {
     __shared__ double scratch[33];
+    __shared__ float tops[33];
     pdl_wait();
+    const long long me = (long long)blockIdx.x * NT + threadIdx.x, all = (long long)gridDim.x * NT;
+    zero_words(a.zeros, a.zero_bytes);
+    if (!a.off.p && a.ref)
+        for (long long i = me; i < a.T; i += all) a.diff[i] = a.logp[i] - a.ref[i];
+    const bool bounded = a.rule.kind != 2;
+    if (bounded && a.weight) {
+        float top = 0.0f;
+        for (long long p = me; p < a.P; p += all) {
+            const float w = fabsf(a.weight[p]);
+            if (w < INFINITY) top = fmaxf(top, w);
+        }
+        top = warp_max(top);
+        if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            top = warp_max(threadIdx.x < NT / 32 ? tops[threadIdx.x] : 0.0f);
+            if (threadIdx.x == 0) a.top[blockIdx.x] = top;
+        }
+    }
+    all_sync<GRID>();
+    float bound = a.rule.beta;
+    if (bounded && a.weight) {
+        float top = 0.0f;
+        for (int i = threadIdx.x & 31; i < (int)gridDim.x; i += 32) top = fmaxf(top, a.top[i]);
+        bound *= warp_max(top);
+    }
+    const GridSums grid_sums(a.grads, bound, 2 * a.P + 1);
+    if (a.off.p) {
+        range_by_seq(a.off, a.S, warp_range(a.T),
+            [&](long long t, bool (&keep)[4], float (&v)[4]) {
+                quad_mask(a.mask, t, a.T, a.whole_mask, keep);
+                quad_load(a.logp, t, a.T, a.whole, 0.0f, v);
+                if (a.ref) {
+                    float r[4];
+                    quad_load(a.ref, t, a.T, a.whole, 0.0f, r);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] -= r[j];
+                }
+            },
+            [&](long long q, double v, int n) {
+                a.scores.add(q, v);
+                atomicAdd(a.count + q, (unsigned long long)n);
+            });
+        all_sync<GRID>();
+    }
     double total = 0.0;
-    for (long long p = (long long)blockIdx.x * PAIR_THREADS + threadIdx.x; p < P;
-         p += (long long)gridDim.x * PAIR_THREADS) {
-        const long long c = chosen.at(p), r = rejected.at(p);
-        const double dc = seq_score(acc, S, c, logp, ref, rule.average);
-        const double dr = seq_score(acc, S, r, logp, ref, rule.average);
-        const PairTerm t = pair_term(rule, (float)(dc - dr));
-        const double w = weight ? (double)weight[p] : 1.0;
-        total += w * (double)t.loss;
-        chosen_reward[p] = (float)(rule.beta * dc);
-        rejected_reward[p] = (float)(rule.beta * dr);
-        const double g = w * (double)t.slope;
-        if (c >= 0 && c < S) acc_add(gacc + c, g);
-        if (r >= 0 && r < S) acc_add(gacc + r, -g);
+    for (long long p0 = me; p0 < a.P; p0 += all * PAIR_EACH) {
+        long long c[PAIR_EACH], r[PAIR_EACH];
+        double dc[PAIR_EACH], dr[PAIR_EACH];
+        float wt[PAIR_EACH];
+#pragma unroll
+        for (int e = 0; e < PAIR_EACH; ++e) {
+            const long long p = p0 + e * all;
+            c[e] = p < a.P ? a.chosen.at(p) : -1;
+            r[e] = p < a.P ? a.rejected.at(p) : -1;
+            wt[e] = a.weight && p < a.P ? a.weight[p] : 1.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < PAIR_EACH; ++e) {
+            dc[e] = seq_score(a, c[e]);
+            dr[e] = seq_score(a, r[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < PAIR_EACH; ++e) {
+            const long long p = p0 + e * all;
+            if (p >= a.P) break;
+            const PairTerm t = pair_term(a.rule, (float)(dc[e] - dr[e]));
+            total += (double)wt[e] * (double)t.loss;
+            a.chosen_reward[p] = (float)(a.rule.beta * dc[e]);
+            a.rejected_reward[p] = (float)(a.rule.beta * dr[e]);
+            const bool in_c = c[e] >= 0 && c[e] < a.S, in_r = r[e] >= 0 && r[e] < a.S;
+            if (bounded) {
+                const float g = wt[e] * t.slope;
+                if (in_c) grid_sums.add(c[e], g);
+                if (in_r) grid_sums.add(r[e], -g);
+            } else {
+                const double g = (double)wt[e] * (double)t.slope;
+                if (in_c) a.grads.add(c[e], g);
+                if (in_r) a.grads.add(r[e], -g);
+            }
+        }
     }
     total = block_sum(total, scratch);
-    if (threadIdx.x == 0) partial[blockIdx.x] = total;
-}
-
-// Gradient of every token: its sequence's, where the token is kept.
-__global__ void __launch_bounds__(TOK_THREADS) k_pref_grad(const uint8_t *mask, long long T, Idx off, long long S,
-                                                           const Acc *acc, const Acc *gacc, long long P, int average,
-                                                           const double *partial, int n_partial, float *loss,
-                                                           float *grad) {
-    __shared__ long long span[2];
-    __shared__ double scratch[33];
-    pdl_wait();
-    const double inv = P ? 1.0 / (double)P : 0.0;
+    if (threadIdx.x == 0) a.partial[blockIdx.x] = total;
+    all_sync<GRID>();
+    const double inv = a.P ? 1.0 / (double)a.P : 0.0;
     if (blockIdx.x == 0) {
         double v = 0.0;
-        for (int i = threadIdx.x; i < n_partial; i += TOK_THREADS) v += partial[i];
+        for (int i = threadIdx.x; i < (int)gridDim.x; i += NT) v += a.partial[i];
         v = block_sum(v, scratch);
-        if (threadIdx.x == 0) *loss = (float)(v * inv);
+        if (threadIdx.x == 0) *a.loss = (float)(v * inv);
     }
-    for (long long t0 = (long long)blockIdx.x * TOK_TILE; t0 < T; t0 += (long long)gridDim.x * TOK_TILE) {
-        const long long t1 = t0 + TOK_TILE < T ? t0 + TOK_TILE : T;
-        if (off.p) tile_span(off, S, t0, t1, span);
-        const long long q0 = off.p ? span[0] : 0, q1 = off.p ? span[1] : 0;
+    auto grad_of = [&](long long q) {
+        const double v = (bounded ? grid_sums.value(q) : a.grads.value(q)) * inv;
+        return (float)(a.rule.average && a.count[q] ? v / (double)a.count[q] : v);
+    };
+    const Range range = warp_range(a.T);
+    const int lane = threadIdx.x & 31;
+    if (!a.off.p) {
+        for (long long t = range.a + lane * 4; t < range.b; t += STEP) {
+            float g[4];
 #pragma unroll
-        for (int e = 0; e < TOK_EACH; ++e) {
-            const long long t = t0 + e * TOK_THREADS + threadIdx.x;
-            if (t >= t1) continue;
-            const long long q = off.p ? token_seq(off, S, q0, q1, t) : t;
-            float g = 0.0f;
-            if (q >= 0 && (!mask || mask[t])) {
-                const double v = acc_value(gacc[q]) * inv;
-                g = (float)(average ? v / (double)acc_count(acc[q]) : v);
-            }
-            grad[t] = g;
+            for (int j = 0; j < 4; ++j) g[j] = t + j < a.T ? grad_of(t + j) : 0.0f;
+            quad_store(a.grad, t, a.T, a.whole, g);
         }
-        __syncthreads();
+        return;
+    }
+    if (range.a >= range.b) return;
+    Place at;
+    at.find(a.off, a.S, 0, range.a);
+    float of = at.valid(a.S) ? grad_of(at.q) : 0.0f;
+    for (long long t0 = range.a; t0 < range.b; t0 += STEP) {
+        const long long t1 = t0 + STEP < range.b ? t0 + STEP : range.b, t = t0 + lane * 4;
+        bool keep[4];
+        float g[4];
+        quad_mask(a.mask, t, a.T, a.whole_mask, keep);
+        if (many_seqs(a.off, a.S, at, t1)) {
+            const long long first = at.q;
+            at.find(a.off, a.S, at.q + 1, t1 - 1);
+            long long q[4];
+            quad_seqs(a.off, a.S, first, at.q, t, q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) g[j] = q[j] < 0 ? 0.0f : j > 0 && q[j] == q[j - 1] ? g[j - 1] : grad_of(q[j]);
+            of = at.valid(a.S) ? grad_of(at.q) : 0.0f;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) g[j] = of;
+            while (at.end < t1) {
+                const long long from = at.end > t0 ? at.end : t0;
+                at.next(a.off, a.S, from);
+                of = at.valid(a.S) ? grad_of(at.q) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (t + j >= from) g[j] = of;
+                if (at.end <= from) break;  // offsets that do not rise
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) g[j] = keep[j] ? g[j] : 0.0f;
+        quad_store(a.grad, t, a.T, a.whole, g);
     }
 }
 
@@ -322,132 +597,237 @@ __device__ __forceinline__ PolicyTerm policy_term(const PolicyRule &r, float log
             p.kl = 0.5f * d * d;
             p.dkl = -d;
         } else {
-            const float e = expm1f(d);
             // e^d - 1 - d loses its digits near zero: Taylor's series there
             // (the term left out is below 2^-24 of the sum)
-            p.kl = fabsf(d) < 0.35f
-                       ? 0.5f * d * d *
-                             fmaf(d * (1.0f / 3), fmaf(d * 0.25f, fmaf(d * 0.2f, fmaf(d * (1.0f / 6),
-                             fmaf(d * (1.0f / 7), fmaf(d, 0.125f, 1.0f), 1.0f), 1.0f), 1.0f), 1.0f), 1.0f)
-                       : e - d;
-            p.dkl = -e;
+            if (fabsf(d) < 0.35f) {
+                p.kl = 0.5f * d * d *
+                       fmaf(d * (1.0f / 3), fmaf(d * 0.25f, fmaf(d * 0.2f, fmaf(d * (1.0f / 6),
+                       fmaf(d * (1.0f / 7), fmaf(d, 0.125f, 1.0f), 1.0f), 1.0f), 1.0f), 1.0f), 1.0f);
+                p.dkl = -(p.kl + d);
+            } else {
+                const float e = expf(d) - 1.0f;
+                p.kl = e - d;
+                p.dkl = -e;
+            }
         }
     }
     return p;
 }
 
-// What the weights of tokens are made from: `total` kept tokens in all, or
-// each sequence's own count (acc[q].n) and the number of sequences with any.
+// What the weights of tokens are made from.
 struct PolicyCount {
-    const unsigned long long *total;  // [0] kept tokens, [1] sequences with kept tokens
-    const Acc *acc;
-    const int *ids;                   // sequence of each row (rows of logits), else null
+    unsigned long long *total;  // [0] kept tokens, [1] sequences with kept tokens
+    unsigned *ticket;           // blocks that have written their share of the loss
+    unsigned long long *count;  // kept tokens by sequence
+    int *ids;                   // sequence of each row (rows of logits), else null
 };
 // In fp32: one rounding of a count and one of the quotient.
 __device__ __forceinline__ float token_weight(const PolicyCount &n) {
     return n.total[0] ? 1.0f / (float)n.total[0] : 0.0f;
 }
 __device__ __forceinline__ float seq_weight(const PolicyCount &n, long long q) {
-    return 1.0f / ((float)acc_count(n.acc[q]) * (float)n.total[1]);
+    return 1.0f / ((float)n.count[q] * (float)n.total[1]);
 }
 
 constexpr int POL_STATS = 4;  // policy term, kl, entropy, clipped
 
-// Counts the kept tokens, in all and (acc not null) by sequence; with `ids` also
-// writes each token's sequence.  A token is kept where mask and label say so
-// and, with offsets, a sequence holds it.
-__global__ void __launch_bounds__(TOK_THREADS) k_policy_count(const uint8_t *mask, Idx labels, long long T, Idx off,
-                                                              long long S, Acc *acc, unsigned long long *total,
-                                                              int *ids) {
-    __shared__ long long span[2];
-    pdl_wait();
-    unsigned mine = 0;
-    for (long long t0 = (long long)blockIdx.x * TOK_TILE; t0 < T; t0 += (long long)gridDim.x * TOK_TILE) {
-        const long long t1 = t0 + TOK_TILE < T ? t0 + TOK_TILE : T;
-        if (off.p) tile_span(off, S, t0, t1, span);
-#pragma unroll
-        for (int e = 0; e < TOK_EACH; ++e) {
-            const long long t = t0 + e * TOK_THREADS + threadIdx.x;
-            bool keep = t < t1 && (!mask || mask[t]) && (!labels.p || labels.at(t) >= 0);
-            if (off.p) {
-                const long long q = t < t1 ? token_seq(off, S, span[0], span[1], t) : -1;
-                if (ids && t < t1) ids[t] = (int)q;
-                keep = keep && q >= 0;
-                if (acc) warp_seq_add(acc, q, 0.0, keep, false);
-            }
-            mine += keep;
-        }
-        __syncthreads();
-    }
-    mine = warp_sum(mine);
-    if ((threadIdx.x & 31) == 0 && mine) atomicAdd(total, (unsigned long long)mine);
-}
-__global__ void k_policy_nonempty(const Acc *acc, long long S, unsigned long long *total) {
-    pdl_wait();
-    unsigned mine = 0;
-    for (long long q = (long long)blockIdx.x * blockDim.x + threadIdx.x; q < S; q += (long long)gridDim.x * blockDim.x)
-        mine += acc_count(acc[q]) != 0;
-    mine = warp_sum(mine);
-    if ((threadIdx.x & 31) == 0 && mine) atomicAdd(total + 1, (unsigned long long)mine);
-}
-
-__device__ __forceinline__ void policy_partial(const double (&sum)[POL_STATS], double *scratch, double *partial) {
-#pragma unroll
-    for (int k = 0; k < POL_STATS; ++k) {
-        const double v = block_sum(sum[k], scratch);
-        if (threadIdx.x == 0) partial[(long long)blockIdx.x * POL_STATS + k] = v;
-    }
-}
-
-__global__ void __launch_bounds__(TOK_THREADS) k_policy_tokens(const float *logp, const float *old, const float *adv,
-                                                               const float *ref, const uint8_t *mask, long long T,
-                                                               Idx off, long long S, PolicyRule rule, PolicyCount cnt,
-                                                               float *grad, double *partial) {
-    __shared__ long long span[2];
-    __shared__ double scratch[33];
-    pdl_wait();
-    double sum[POL_STATS] = {};
-    const float w_all = rule.by_sequence ? 0.0f : token_weight(cnt);
-    for (long long t0 = (long long)blockIdx.x * TOK_TILE; t0 < T; t0 += (long long)gridDim.x * TOK_TILE) {
-        const long long t1 = t0 + TOK_TILE < T ? t0 + TOK_TILE : T;
-        if (off.p) tile_span(off, S, t0, t1, span);
-#pragma unroll
-        for (int e = 0; e < TOK_EACH; ++e) {
-            const long long t = t0 + e * TOK_THREADS + threadIdx.x;
-            if (t >= t1) continue;
-            const long long q = off.p ? token_seq(off, S, span[0], span[1], t) : -1;
-            float g = 0.0f;
-            if ((!mask || mask[t]) && (q >= 0 || !(rule.by_sequence || rule.adv_by_sequence))) {
-                const float w = rule.by_sequence ? seq_weight(cnt, q) : w_all;
-                const PolicyTerm p = policy_term(rule, logp[t], old[t], adv[rule.adv_by_sequence ? q : t],
-                                                 rule.kl_kind ? ref[t] : 0.0f);
-                g = w * (rule.kl_coef != 0.0f ? fmaf(rule.kl_coef, p.dkl, p.dpg) : p.dpg);
-                sum[0] += (double)w * p.pg;
-                sum[1] += (double)w * p.kl;
-                sum[3] += (double)w * p.cut;
-            }
-            grad[t] = g;
-        }
-        __syncthreads();
-    }
-    policy_partial(sum, scratch, partial);
-}
-
-// stats: loss, policy term, kl, entropy, share clipped (weighted means)
-__global__ void k_policy_finish(const double *partial, int blocks, PolicyRule rule, float *stats) {
-    __shared__ double scratch[33];
-    pdl_wait();
-    double sum[POL_STATS] = {};
-    for (int i = threadIdx.x; i < blocks; i += blockDim.x)
-        for (int k = 0; k < POL_STATS; ++k) sum[k] += partial[(long long)i * POL_STATS + k];
-    for (int k = 0; k < POL_STATS; ++k) sum[k] = block_sum(sum[k], scratch);
-    if (threadIdx.x == 0) {
-        double loss = sum[0];
-        if (rule.kl_coef != 0.0f) loss += (double)rule.kl_coef * sum[1];
-        if (rule.ent_coef != 0.0f) loss -= (double)rule.ent_coef * sum[2];
+// The block's sums into its place of `partial`; the last block to come adds all
+// blocks' up, in their order, to stats: loss, policy term, kl, entropy, share
+// clipped.  `sum` counts in lane 0; one warp calls it.
+__device__ __forceinline__ void policy_end(const double *sum, const PolicyRule &rule, unsigned *ticket, double *partial,
+                                           float *stats) {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0)
+        for (int k = 0; k < POL_STATS; ++k) partial[(long long)blockIdx.x * POL_STATS + k] = sum[k];
+    if (!last_of_grid(ticket)) return;
+    double all[POL_STATS] = {};
+    for (int i = lane; i < (int)gridDim.x; i += 32)
+        for (int k = 0; k < POL_STATS; ++k) all[k] += __ldcg(partial + (long long)i * POL_STATS + k);
+    for (int k = 0; k < POL_STATS; ++k) all[k] = warp_sum(all[k]);
+    if (lane == 0) {
+        double loss = all[0];
+        if (rule.kl_coef != 0.0f) loss += (double)rule.kl_coef * all[1];
+        if (rule.ent_coef != 0.0f) loss -= (double)rule.ent_coef * all[2];
         stats[0] = (float)loss;
-        for (int k = 0; k < POL_STATS; ++k) stats[1 + k] = (float)sum[k];
+        for (int k = 0; k < POL_STATS; ++k) stats[1 + k] = (float)all[k];
     }
+}
+// The same by a whole block, every thread with sums of its own.
+__device__ __forceinline__ void policy_end_block(double (&sum)[POL_STATS], const PolicyRule &rule, unsigned *ticket,
+                                                 double *partial, float *stats, double *scratch /* >= 33 */) {
+    for (int k = 0; k < POL_STATS; ++k) sum[k] = block_sum(sum[k], scratch);
+    if (threadIdx.x < 32) policy_end(sum, rule, ticket, partial, stats);
+}
+
+struct CountArgs {
+    const uint8_t *mask;
+    Idx labels;  // null: no labels
+    long long T;
+    Idx off;     // null: no sequences
+    long long S;
+    bool by_sequence, whole_mask;
+    PolicyCount cnt;
+    long long zero_bytes;  // from cnt.total on
+};
+
+// Counts the kept tokens, in all and by sequence; with ids also writes each
+// token's sequence.  A token is kept where mask and label say so and, with
+// offsets, a sequence holds it.
+template <int NT>
+__device__ __forceinline__ void policy_count(const CountArgs &a, double *scratch) {
+    long long kept = 0, full = 0;
+    const Range r = warp_range(a.T);
+    auto fetch = [&](long long t, bool (&keep)[4], float (&v)[4]) {
+        quad_mask(a.mask, t, a.T, a.whole_mask, keep);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (a.labels.p) keep[j] = keep[j] && a.labels.at(t + j) >= 0;  // keep: t + j < T
+            v[j] = 0.0f;
+        }
+    };
+    if (a.off.p) {
+        range_by_seq(a.off, a.S, r, fetch, [&](long long q, double, int n) {
+            if (a.by_sequence) full += atomicAdd(a.cnt.count + q, (unsigned long long)n) == 0;
+            kept += n;
+        });
+        if (a.cnt.ids && r.a < r.b) {
+            Place at;
+            at.find(a.off, a.S, 0, r.a);
+            const long long first = at.q;
+            at.find(a.off, a.S, 0, r.b - 1);
+            for (long long t = r.a + (threadIdx.x & 31) * 4; t < r.b; t += STEP) {
+                long long q[4];
+                quad_seqs(a.off, a.S, first, at.q, t, q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (t + j < r.b) a.cnt.ids[t + j] = (int)q[j];
+            }
+        }
+    } else {
+        for (long long t = r.a + (threadIdx.x & 31) * 4; t < r.b; t += STEP) {
+            bool keep[4];
+            float none[4];
+            fetch(t, keep, none);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) kept += keep[j] && t + j < r.b;
+        }
+    }
+    // whole numbers below 2^53: exact as double
+    const double k = block_sum((double)kept, scratch), f = block_sum((double)full, scratch);
+    if (threadIdx.x == 0) {
+        if (k > 0) atomicAdd(a.cnt.total, (unsigned long long)k);
+        if (f > 0) atomicAdd(a.cnt.total + 1, (unsigned long long)f);
+    }
+}
+template <bool GRID, int NT>
+__global__ void __launch_bounds__(NT) k_policy_count(const __grid_constant__ CountArgs a) {
+    __shared__ double scratch[33];
+    pdl_wait();
+    zero_words(a.cnt.total, a.zero_bytes);
+    all_sync<GRID>();
+    policy_count<NT>(a, scratch);
+}
+
+struct PolicyTokens {
+    CountArgs count;  // its labels are null
+    const float *logp, *old, *adv, *ref;
+    PolicyRule rule;
+    float *grad, *stats;
+    double *partial;
+    bool whole;
+};
+// Bytes: 17 a token read (and its mask byte twice), 4 written.
+template <bool GRID, int NT>
+__global__ void __launch_bounds__(NT) k_policy_tokens(const __grid_constant__ PolicyTokens a) {
+    __shared__ double scratch[33];
+    pdl_wait();
+    const CountArgs &n = a.count;
+    zero_words(n.cnt.total, n.zero_bytes);
+    all_sync<GRID>();
+    policy_count<NT>(n, scratch);
+    all_sync<GRID>();
+    double sum[POL_STATS] = {};
+    const PolicyRule &rule = a.rule;
+    const float w_all = rule.by_sequence ? 0.0f : token_weight(n.cnt);
+    const Range r = warp_range(n.T);
+    const int lane = threadIdx.x & 31;
+    Place at{0, LLONG_MAX};
+    float wt = w_all, av = 0.0f;  // of the sequence that the warp is in
+    bool in = true;
+    auto weight_of = [&](long long q) { return rule.by_sequence && n.cnt.count[q] ? seq_weight(n.cnt, q) : w_all; };
+    auto enter = [&]() {
+        in = at.valid(n.S);
+        wt = in ? weight_of(at.q) : 0.0f;
+        av = in && rule.adv_by_sequence ? a.adv[at.q] : 0.0f;
+    };
+    if (n.off.p && r.a < r.b) {
+        at.find(n.off, n.S, 0, r.a);
+        enter();
+    }
+    for (long long t0 = r.a; t0 < r.b; t0 += STEP) {
+        const long long t1 = t0 + STEP < r.b ? t0 + STEP : r.b, t = t0 + lane * 4;
+        bool keep[4];
+        float x[4], old[4], adv[4] = {av, av, av, av}, w[4] = {wt, wt, wt, wt}, ref[4] = {0.0f, 0.0f, 0.0f, 0.0f}, g[4];
+        quad_mask(n.mask, t, n.T, n.whole_mask, keep);
+        quad_load(a.logp, t, n.T, a.whole, 0.0f, x);
+        quad_load(a.old, t, n.T, a.whole, 0.0f, old);
+        if (!rule.adv_by_sequence) quad_load(a.adv, t, n.T, a.whole, 0.0f, adv);
+        if (rule.kl_kind) quad_load(a.ref, t, n.T, a.whole, 0.0f, ref);
+        if (at.end >= t1) {  // one sequence
+#pragma unroll
+            for (int j = 0; j < 4; ++j) keep[j] = keep[j] && in;
+        } else if (many_seqs(n.off, n.S, at, t1)) {
+            const long long first = at.q;
+            at.find(n.off, n.S, at.q + 1, t1 - 1);
+            long long q[4];
+            quad_seqs(n.off, n.S, first, at.q, t, q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                keep[j] = keep[j] && q[j] >= 0;
+                if (j > 0 && q[j] == q[j - 1]) {
+                    w[j] = w[j - 1];
+                    if (rule.adv_by_sequence) adv[j] = adv[j - 1];
+                } else if (q[j] >= 0) {
+                    w[j] = weight_of(q[j]);
+                    if (rule.adv_by_sequence) adv[j] = a.adv[q[j]];
+                }
+            }
+            enter();
+        } else {
+            bool held[4] = {in, in, in, in};
+            while (at.end < t1) {
+                const long long from = at.end > t0 ? at.end : t0;
+                at.next(n.off, n.S, from);
+                enter();
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (t + j >= from) {
+                        held[j] = in;
+                        w[j] = wt;
+                        if (rule.adv_by_sequence) adv[j] = av;
+                    }
+                if (at.end <= from) break;  // offsets that do not rise
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) keep[j] = keep[j] && held[j];
+        }
+        float s0 = 0.0f, s1 = 0.0f, s3 = 0.0f;  // of four tokens
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const PolicyTerm p = policy_term(rule, x[j], old[j], adv[j], ref[j]);
+            g[j] = keep[j] ? w[j] * (rule.kl_coef != 0.0f ? fmaf(rule.kl_coef, p.dkl, p.dpg) : p.dpg) : 0.0f;
+            if (keep[j]) {
+                s0 = fmaf(w[j], p.pg, s0);
+                s1 = fmaf(w[j], p.kl, s1);
+                s3 = fmaf(w[j], p.cut, s3);
+            }
+        }
+        sum[0] += (double)s0;
+        sum[1] += (double)s1;
+        sum[3] += (double)s3;
+        quad_store(a.grad, t, n.T, a.whole, g);
+    }
+    policy_end_block(sum, rule, n.cnt.ticket, a.partial, a.stats, scratch);
 }
 
 // ---------------------------------------------------------------- host --
@@ -468,6 +848,34 @@ static inline int grid_of(long long items, long long per_block, int most) {
 }
 static inline long long round_up256(long long b) { return (b + 255) & ~255ll; }
 
+// Resident clusters (or blocks) of a kernel on the current device.
+template <typename K>
+static int resident(K kernel, int nt, int cl, int smem, int (&cache)[64]) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sm_count();
+    if (!cache[dev]) {
+        int n = 0;
+        if (cl == 1) {
+            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, nt, smem) != cudaSuccess) n = 0;
+            n *= sm_count();
+        } else {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(cl);
+            cfg.blockDim = dim3(nt);
+            cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = cl;
+            at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+            cfg.attrs = at;
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
+        }
+        cache[dev] = n > 0 ? n : 1;
+    }
+    return cache[dev];
+}
+
 static int check_index(const char *name, int bytes) {
     WGB_CHECK_ARG(bytes == 4 || bytes == 8, "%s must be 4- or 8-byte integers", name);
     return WGB_OK;
@@ -478,13 +886,80 @@ static int check_index(const char *name, int bytes) {
         if (rc_ != WGB_OK) return rc_;    \
     } while (0)
 
+
+// Launches `kernel<true, 256>` over all SMs as a cooperative grid, or
+// `kernel<false, 1024>` as one block for at most ONE_BLOCK tokens' worth of work,
+// which a block does in the time of a grid's barriers.
+constexpr long long ONE_BLOCK = 16384;
+constexpr int GRID_THREADS = 256, BLOCK_THREADS = 1024;
+constexpr int MAX_BLOCKS_PER_SM = 8;
+template <typename A>
+static int launch_all(const char *name, void (*grid_kernel)(A), void (*block_kernel)(A), long long work, int (&cache)[64],
+                      const A &args, cudaStream_t st) {
+    if (work <= ONE_BLOCK) {
+        WGB_PDL(name, block_kernel, dim3(1), dim3(BLOCK_THREADS), 0, st, args);
+        return WGB_OK;
+    }
+    long long most = resident(grid_kernel, GRID_THREADS, 1, 0, cache);
+    if (most > (long long)sm_count() * MAX_BLOCKS_PER_SM) most = (long long)sm_count() * MAX_BLOCKS_PER_SM;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid_of(work, GRID_THREADS * 4, (int)most));
+    cfg.blockDim = dim3(GRID_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeCooperative;
+    at[0].val.cooperative = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, grid_kernel, args);
+    if (e != cudaSuccess) {
+        set_error("launch of %s failed: %s", name, cudaGetErrorString(e));
+        return WGB_ERR_CUDA;
+    }
+    return WGB_OK;
+}
+static bool on16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+static bool on4(const void *p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
+
 }  // namespace wgb
 
 using namespace wgb;
 
+namespace wgb {
+struct PrefWs {
+    double *partial;
+    char *zeros;
+    long long zero_bytes, bytes;
+    Sums grads, scores;
+    unsigned long long *count;
+    float *top, *diff;
+};
+static PrefWs pref_ws(void *ws, long long sequences, bool ragged) {
+    PrefWs w;
+    char *p = static_cast<char *>(ws);
+    w.partial = reinterpret_cast<double *>(p);
+    long long at = round_up256((long long)sm_count() * MAX_BLOCKS_PER_SM * sizeof(double));
+    w.top = reinterpret_cast<float *>(p + at);
+    at += round_up256((long long)sm_count() * MAX_BLOCKS_PER_SM * sizeof(float));
+    w.zeros = p + at;
+    const long long from = at, one = sums_bytes(sequences);
+    w.grads = sums_at(p + at, sequences);
+    at += one;
+    w.scores = sums_at(p + at, sequences);
+    if (ragged) at += one;
+    w.count = reinterpret_cast<unsigned long long *>(p + at);
+    if (ragged) at += (sequences + 1) / 2 * 16;
+    w.zero_bytes = at - from;
+    w.diff = reinterpret_cast<float *>(p + at);
+    if (!ragged) at += 4 * sequences;
+    w.bytes = round_up256(at);
+    return w;
+}
+}  // namespace wgb
+
 extern "C" int64_t wgb_preference_ws_bytes(int64_t sequences, int32_t ragged) {
     if (sequences < 0) return 0;
-    return round_up256((ragged ? 2 : 1) * sequences * (int64_t)sizeof(Acc)) + PAIR_BLOCKS * (int64_t)sizeof(double);
+    return pref_ws(nullptr, sequences, ragged != 0).bytes;
 }
 
 extern "C" int wgb_preference_loss(const float *logp, const float *ref_logp, int64_t tokens, const void *offsets,
@@ -507,46 +982,57 @@ extern "C" int wgb_preference_loss(const float *logp, const float *ref_logp, int
     WGB_CHECK_ARG(loss != nullptr, "loss must not be null");
     WGB_CHECK_ARG(ws && ws_bytes >= wgb_preference_ws_bytes(sequences, offsets != nullptr), "workspace too small");
     WGB_CHECK_ARG(reinterpret_cast<uintptr_t>(ws) % 16 == 0, "workspace is not aligned to 16 bytes");
-    cudaStream_t st = as_stream(stream);
-    Acc *gacc = static_cast<Acc *>(ws);
-    Acc *acc = offsets ? gacc + sequences : nullptr;
-    const long long n_acc = (offsets ? 2 : 1) * sequences;
-    double *partial = reinterpret_cast<double *>(static_cast<char *>(ws) + round_up256(n_acc * (long long)sizeof(Acc)));
-    const Idx off{offsets, offset_bytes == 8}, ci{chosen, index_bytes == 8}, ri{rejected, index_bytes == 8};
-    const PairRule rule{kind, beta, smoothing, average};
-    const int tok_grid = grid_of(tokens, TOK_TILE, sm_count() * 8);
-    if (n_acc)
-        WGB_PDL("k_acc_zero", k_acc_zero, dim3((unsigned)((n_acc + 255) / 256)), dim3(256), 0, st, gacc, n_acc,
-                (unsigned long long *)nullptr, 0);
-    if (offsets && tokens)
-        WGB_PDL("k_pref_sums", k_pref_sums, dim3(tok_grid), dim3(TOK_THREADS), 0, st, logp, ref_logp, mask, tokens, off,
-                sequences, acc);
-    const int pair_grid = grid_of(pairs, PAIR_THREADS, PAIR_BLOCKS);
-    WGB_PDL("k_pref_pairs", k_pref_pairs, dim3(pair_grid), dim3(PAIR_THREADS), 0, st, logp, ref_logp,
-            (const Acc *)acc, sequences, ci, ri, pairs, weight, rule, gacc, chosen_reward, rejected_reward, partial);
-    WGB_PDL("k_pref_grad", k_pref_grad, dim3(tok_grid), dim3(TOK_THREADS), 0, st, mask, tokens, off, sequences,
-            (const Acc *)acc, (const Acc *)gacc, pairs, average, (const double *)partial, pair_grid, loss, grad_logp);
-    return WGB_OK;
+    const PrefWs w = pref_ws(ws, sequences, offsets != nullptr);
+    PrefArgs a = {};
+    a.logp = logp;
+    a.ref = ref_logp;
+    a.T = tokens;
+    a.off = Idx{offsets, offset_bytes == 8};
+    a.S = sequences;
+    a.mask = mask;
+    a.chosen = Idx{chosen, index_bytes == 8};
+    a.rejected = Idx{rejected, index_bytes == 8};
+    a.P = pairs;
+    a.weight = weight;
+    a.rule = PairRule{kind, beta, smoothing, average};
+    a.loss = loss;
+    a.grad = grad_logp;
+    a.chosen_reward = chosen_reward;
+    a.rejected_reward = rejected_reward;
+    a.partial = w.partial;
+    a.zeros = w.zeros;
+    a.zero_bytes = w.zero_bytes;
+    a.grads = w.grads;
+    a.scores = w.scores;
+    a.count = w.count;
+    a.top = w.top;
+    a.diff = w.diff;
+    a.whole = on16(logp) && on16(ref_logp) && on16(grad_logp);
+    a.whole_mask = on4(mask);
+    static int cache[64];
+    // a pair costs about as much as four tokens, a sequence as two
+    return launch_all("k_preference", k_preference<true, GRID_THREADS>, k_preference<false, BLOCK_THREADS>,
+                      tokens + 4 * pairs + 2 * sequences, cache, a, as_stream(stream));
 }
 
 namespace wgb {
 constexpr int POL_BLOCKS_PER_SM = 16;
 struct PolicyWs {
-    unsigned long long *total;
+    PolicyCount cnt;
     double *partial;
-    Acc *acc;
-    int *ids;
-    long long bytes;
+    long long zero_bytes, bytes;
 };
 static PolicyWs policy_ws(void *ws, long long tokens, long long sequences, bool ids) {
     PolicyWs w;
     char *p = static_cast<char *>(ws);
-    w.total = reinterpret_cast<unsigned long long *>(p);
-    w.partial = reinterpret_cast<double *>(p + 256);
-    long long at = 256 + round_up256((long long)sm_count() * POL_BLOCKS_PER_SM * POL_STATS * sizeof(double));
-    w.acc = reinterpret_cast<Acc *>(p + at);
-    at += round_up256(sequences * (long long)sizeof(Acc));
-    w.ids = ids ? reinterpret_cast<int *>(p + at) : nullptr;
+    w.cnt.total = reinterpret_cast<unsigned long long *>(p);
+    w.cnt.ticket = reinterpret_cast<unsigned *>(p + 16);
+    w.cnt.count = reinterpret_cast<unsigned long long *>(p + 32);
+    w.zero_bytes = 32 + (sequences + 1) / 2 * 16;
+    long long at = round_up256(w.zero_bytes);
+    w.partial = reinterpret_cast<double *>(p + at);
+    at += round_up256((long long)sm_count() * POL_BLOCKS_PER_SM * POL_STATS * sizeof(double));
+    w.cnt.ids = ids ? reinterpret_cast<int *>(p + at) : nullptr;
     w.bytes = at + (ids ? round_up256(tokens * 4) : 0);
     return w;
 }
@@ -575,17 +1061,10 @@ static int policy_rule(const PolicyArgs &a, const float *ref, long long tokens, 
     return WGB_OK;
 }
 
-// Zeroes and counts what the weights need.
-static int policy_counts(const PolicyWs &w, const uint8_t *mask, Idx labels, long long tokens, Idx off,
-                         long long sequences, const PolicyRule &rule, cudaStream_t st) {
-    const long long n = rule.by_sequence ? sequences : 0;
-    WGB_PDL("k_acc_zero", k_acc_zero, dim3((unsigned)((n + 255) / 256 + (n == 0))), dim3(256), 0, st, w.acc, n, w.total, 2);
-    WGB_PDL("k_policy_count", k_policy_count, dim3(grid_of(tokens, TOK_TILE, sm_count() * 8)), dim3(TOK_THREADS), 0, st,
-            mask, labels, tokens, off, sequences, rule.by_sequence ? w.acc : nullptr, w.total, w.ids);
-    if (rule.by_sequence)
-        WGB_PDL("k_policy_nonempty", k_policy_nonempty, dim3(grid_of(sequences, 256, sm_count())), dim3(256), 0, st,
-                (const Acc *)w.acc, sequences, w.total);
-    return WGB_OK;
+static CountArgs count_args(const PolicyWs &w, const uint8_t *mask, Idx labels, long long tokens, Idx off,
+                            long long sequences, const PolicyRule &rule) {
+    return CountArgs{mask,   labels, tokens, off, sequences, rule.by_sequence != 0, on4(mask),
+                     w.cnt,  rule.by_sequence ? w.zero_bytes : 32};
 }
 }  // namespace wgb
 
@@ -610,15 +1089,20 @@ extern "C" int wgb_policy_loss(const float *logp, const float *old_logp, const f
     WGB_CHECK_ARG(stats != nullptr, "stats must not be null");
     WGB_CHECK_ARG(ws && ws_bytes >= wgb_policy_ws_bytes(tokens, sequences, 0), "workspace too small");
     WGB_CHECK_ARG(reinterpret_cast<uintptr_t>(ws) % 16 == 0, "workspace is not aligned to 16 bytes");
-    cudaStream_t st = as_stream(stream);
     const PolicyWs w = policy_ws(ws, tokens, sequences, false);
     const bool seqs = by_sequence || adv_by_sequence;
-    const Idx off{seqs ? offsets : nullptr, offset_bytes == 8};
-    WGB_TRY(policy_counts(w, mask, Idx{nullptr, 0}, tokens, off, sequences, rule, st));
-    const int grid = grid_of(tokens, TOK_TILE, sm_count() * POL_BLOCKS_PER_SM);
-    WGB_PDL("k_policy_tokens", k_policy_tokens, dim3(grid), dim3(TOK_THREADS), 0, st, logp, old_logp, advantages,
-            ref_logp, mask, tokens, off, sequences, rule, PolicyCount{w.total, w.acc, nullptr}, grad_logp, w.partial);
-    WGB_PDL("k_policy_finish", k_policy_finish, dim3(1), dim3(256), 0, st, (const double *)w.partial, grid, rule, stats);
-    return WGB_OK;
+    PolicyTokens a = {};
+    a.count = count_args(w, mask, Idx{nullptr, 0}, tokens, Idx{seqs ? offsets : nullptr, offset_bytes == 8}, sequences, rule);
+    a.logp = logp;
+    a.old = old_logp;
+    a.adv = advantages;
+    a.ref = ref_logp;
+    a.rule = rule;
+    a.grad = grad_logp;
+    a.stats = stats;
+    a.partial = w.partial;
+    a.whole = on16(logp) && on16(old_logp) && (adv_by_sequence || on16(advantages)) && on16(ref_logp) && on16(grad_logp);
+    static int cache[64];
+    return launch_all("k_policy_tokens", k_policy_tokens<true, GRID_THREADS>, k_policy_tokens<false, BLOCK_THREADS>,
+                      tokens + (by_sequence ? sequences : 0), cache, a, as_stream(stream));
 }
-
