@@ -587,16 +587,15 @@ __device__ __forceinline__ RowRaw row_seen(const RowsArgs &a, long long i) {
     if (i >= a.rows) return r;
     r.y = a.labels.at(i);
     if (OP == ROW_POLICY && a.mask) r.mask = a.mask[i];
-    if (OP == ROW_POLICY && a.cnt.ids) r.q = a.cnt.ids[i];
     return r;
 }
 __device__ __forceinline__ int label_of(const RowRaw &r, long long K) { return (int)(r.y < 0 ? -1 : r.y < K ? r.y : K); }
-__device__ __forceinline__ bool row_kept(const RowRaw &r) { return r.y >= 0 && r.mask != 0 && r.q >= 0; }
+// What label and mask say; a row is kept if a sequence holds it too.
+__device__ __forceinline__ bool row_passes(const RowRaw &r) { return r.y >= 0 && r.mask != 0; }
 template <int OP>
-__device__ __forceinline__ RowIn row_open(const RowsArgs &a, const RowRaw &r, float w_all) {
-    RowIn in{label_of(r, a.K), row_kept(r), r.a0, r.a1, r.a2, r.a3};
+__device__ __forceinline__ RowIn row_open(const RowsArgs &a, const RowRaw &r) {
+    RowIn in{label_of(r, a.K), row_passes(r) && r.q >= 0, r.a0, r.a1, r.a2, r.a3};
     if (OP == ROW_POLICY) {
-        in.a3 = w_all;
         if (in.kept && a.rule.adv_by_sequence) in.a1 = a.adv[r.q];
         if (in.kept && a.rule.by_sequence) in.a3 = seq_weight(a.cnt, r.q);
     }
@@ -652,10 +651,28 @@ __device__ __forceinline__ RowGrad row_close(const RowsArgs &a, const RowIn &in,
     }
     return r;
 }
+// The policy step's kernel is launched while the kernel that counts its tokens
+// still runs (everything before that one is done): it reads rows at once and
+// waits for the counts when it needs them.  Sequences it needs from the start.
 template <int OP>
-__device__ __forceinline__ float row_weight_all(const RowsArgs &a) {
-    return OP == ROW_POLICY && !a.rule.by_sequence ? token_weight(a.cnt) : 0.0f;
+__device__ __forceinline__ void early_wait(const RowsArgs &a) {
+    if (OP != ROW_POLICY || a.cnt.ids) pdl_wait();
 }
+template <int OP>
+struct LateWeight {
+    bool known = false;
+    float w = 0.0f;
+    // Full warps call it.
+    __device__ __forceinline__ void set(const RowsArgs &a, RowIn &in) {
+        if (OP != ROW_POLICY || a.rule.by_sequence) return;
+        if (!known) {
+            pdl_wait();
+            w = token_weight(a.cnt);
+            known = true;
+        }
+        in.a3 = w;
+    }
+};
 template <typename T>
 __device__ __forceinline__ float label_logit(const T *row, const RowIn &in, long long K) {
     return in.kept && in.y < K ? Vec<T>::to(row[in.y]) : NAN;
@@ -686,7 +703,7 @@ __global__ void __launch_bounds__(NT, GL > 32 ? 1024 / NT : 4) k_rows(const __gr
     constexpr bool SENT = ENT && OP != ROW_GRAD;  // the sums have an entropy
     __shared__ float4 part[2][BLOCK ? NT / 32 : 1], again[BLOCK ? NT / 32 : 1];
     __shared__ double dscratch[33];
-    pdl_wait();
+    early_wait<OP>(a);
     __shared__ double shared_tot[POL_STATS];  // a block's one leader keeps its totals out of the registers
     double own_tot[POL_STATS] = {};
     double *tot = BLOCK ? shared_tot : own_tot;
@@ -696,7 +713,7 @@ __global__ void __launch_bounds__(NT, GL > 32 ? 1024 / NT : 4) k_rows(const __gr
     T *grad = static_cast<T *>(a.grad);
     const int tid = BLOCK ? threadIdx.x : threadIdx.x % GL;
     const float inv_t = 1.0f / a.temperature, c = (float)LOG2E * inv_t;
-    const float w_all = row_weight_all<OP>(a);
+    LateWeight<OP> weight;
     const long long step = (long long)gridDim.x * RPC;
     int turn = 0;
     const long long mine = (long long)blockIdx.x * RPC + (BLOCK ? 0 : threadIdx.x / GL);
@@ -704,7 +721,7 @@ __global__ void __launch_bounds__(NT, GL > 32 ? 1024 / NT : 4) k_rows(const __gr
     for (long long base = (long long)blockIdx.x * RPC; base < a.rows; base += step) {
         const long long i = base + (BLOCK ? 0 : threadIdx.x / GL);
         const bool live = i < a.rows;
-        const RowIn in = row_open<OP>(a, next, w_all);
+        RowIn in = row_open<OP>(a, next);
         const T *row = logits + (live ? i : 0) * a.stride;
         T *out = OP == ROW_LOGP ? nullptr : grad + (live ? i : 0) * a.grad_stride;
         const RowWords<T, int> rw(row, OP == ROW_LOGP ? row : out, (int)a.K);
@@ -734,6 +751,7 @@ __global__ void __launch_bounds__(NT, GL > 32 ? 1024 / NT : 4) k_rows(const __gr
             row_mend<T, GL, NT, SENT>(sum, scaled, row, a.K, in.kept, tid, c, again);
             careful = Vec<T>::HALF && in.kept && !scaled;
         }
+        weight.set(a, in);
         const RowGrad r = row_close<OP, ENT>(a, in, sum, summed, scaled, x_y, i, live && tid == 0, inv_t, c, tot);
         if (!BLOCK) __syncwarp();  // in place: every lane has read its row before any writes
         if (OP != ROW_LOGP && live) {
@@ -770,10 +788,11 @@ __global__ void __launch_bounds__(NT, 2) k_rows_long(const __grid_constant__ Row
     T *grad = static_cast<T *>(a.grad);
     const int tid = threadIdx.x;
     const float inv_t = 1.0f / a.temperature, c = (float)LOG2E * inv_t;
-    const float w_all = row_weight_all<OP>(a);
+    LateWeight<OP> weight;
     int turn = 0;
     for (long long i = blockIdx.x; i < a.rows; i += gridDim.x) {
-        const RowIn in = row_open<OP>(a, row_fetch<OP>(a, i), w_all);
+        RowIn in = row_open<OP>(a, row_fetch<OP>(a, i));
+        weight.set(a, in);
         const T *row = logits + i * a.stride;
         T *out = OP == ROW_LOGP ? nullptr : grad + i * a.grad_stride;
         const RowWords<T, long long> rw(row, OP == ROW_LOGP ? row : out, a.K);
@@ -913,7 +932,7 @@ __global__ void __launch_bounds__(RING_NT, ring_blocks<OP>()) k_rows_ring(const 
     }
     if (CL > 1) cluster_sync();
     else __syncthreads();
-    pdl_wait();
+    if (OP != ROW_POLICY || warp == RING_WARPS + 1) pdl_wait();  // the counts matter to the closing warp alone
     const T *logits = static_cast<const T *>(a.logits);
     T *grad = static_cast<T *>(a.grad);
     const int K = (int)a.K;
@@ -933,10 +952,10 @@ __global__ void __launch_bounds__(RING_NT, ring_blocks<OP>()) k_rows_ring(const 
             }
         };
         for (long long i = row0; i < a.rows && !lost; i += step) {
-            const bool kept = row_kept(after);
+            const bool through = row_passes(after);
             const int y = label_of(after, a.K);
             after = row_seen<OP>(a, i + step);
-            if (!kept) continue;
+            if (!through) continue;
             const T *row = logits + i * a.stride;
             const RowRec r = row_rec<T, CL>(row, K, i, y, rank);
             const T *src = row + r.head + (long long)r.begin * N;
@@ -959,14 +978,16 @@ __global__ void __launch_bounds__(RING_NT, ring_blocks<OP>()) k_rows_ring(const 
             bar_arrive(&full[slot]);
         }
     } else if (warp == RING_WARPS + 1) {  // -------------------------- closing
-        const float w_all = row_weight_all<OP>(a);
+        LateWeight<OP> weight;
         double tot[POL_STATS] = {};
         RowRaw next = row_fetch<OP>(a, row0);
         int k = 0;
         unsigned mends = 0;
         // ROW_LOGP: rank 0 closes for the whole cluster
         for (long long i = OP == ROW_LOGP && rank > 0 ? a.rows : row0; i < a.rows; i += step) {
-            const RowIn in = row_open<OP>(a, next, w_all);
+            const bool through = row_passes(next);  // its words come through the ring
+            RowIn in = row_open<OP>(a, next);
+            weight.set(a, in);
             next = row_fetch<OP>(a, i + step);
             const T *row = logits + i * a.stride;
             T *out = OP == ROW_LOGP ? nullptr : grad + i * a.grad_stride;
@@ -975,7 +996,7 @@ __global__ void __launch_bounds__(RING_NT, ring_blocks<OP>()) k_rows_ring(const 
             RowSum sum = row_none();
             bool scaled = false;
             const bool resum = OP == ROW_GRAD && row_resum(in);
-            if (in.kept && OP != ROW_GRAD) {
+            if (through && OP != ROW_GRAD) {
                 bar_wait(&joined[k & 1], (k >> 1) & 1, lost);
                 sum = entries_join<CL * RING_WARPS, SENT>(part[k & 1], HALF ? 1.0f : c);
                 x_y = part[k & 1][0].w;
@@ -996,7 +1017,7 @@ __global__ void __launch_bounds__(RING_NT, ring_blocks<OP>()) k_rows_ring(const 
                                            c, tot);
             r.careful = resum || (HALF && in.kept && OP != ROW_GRAD && !scaled);
             if (lost) r.b = r.b2 = NAN;
-            if (in.kept) {
+            if (through) {
                 if (OP == ROW_GRAD && k >= 2) bar_wait(&taken[k & 1], ((k >> 1) - 1) & 1, lost);
                 __syncwarp();  // all lanes have read the entries
                 if (CL > 1 && OP != ROW_GRAD && lane == 0) bar_expect(&joined[k & 1], CL * RING_WARPS * 16);  // of row k + 2
@@ -1010,8 +1031,8 @@ __global__ void __launch_bounds__(RING_NT, ring_blocks<OP>()) k_rows_ring(const 
                 ++k;
             }
             if (OP != ROW_LOGP) {
-                if (!in.kept || lost) {  // a row that is left out: zeros
-                    const float v = in.kept ? NAN : 0.0f;
+                if (!through || lost) {  // a row that is left out: zeros
+                    const float v = through ? NAN : 0.0f;
                     const float f[8] = {v, v, v, v, v, v, v, v};
                     const uint4 z = Vec<T>::pack(*reinterpret_cast<const float(*)[N]>(f));
                     uint4 *o = reinterpret_cast<uint4 *>(out + rec.head) + rec.begin;
@@ -1138,79 +1159,104 @@ __global__ void __launch_bounds__(RING_NT, ring_blocks<OP>()) k_rows_ring(const 
 }
 
 // Rows of few classes: a thread to a row.  A block stages TILE_ROWS rows in
-// shared memory as fp32 (pitch odd, so that the threads' columns lie in
-// different banks), which makes the loads and stores of HBM consecutive
-// whatever the number of classes.
+// shared memory as they lie, one after another, so that HBM sees consecutive
+// words whatever the number of classes; a thread then holds its row in KM
+// registers.  Threads t and t + 32 / g (g the power of two in a row's 4-byte
+// words) would meet in the same bank, so each such group starts its row at an
+// element of its own.
 constexpr int TILE_ROWS = 128;
 constexpr int TILE_CLASSES = 32;
-constexpr int TILE_BATCH = 8;  // loads in flight
 
-template <typename T, int OP, bool ENT>
+// Moves n elements between shared memory and consecutive global memory.
+template <typename T>
+__device__ __forceinline__ void tile_in(T *tile, const T *from, int n, bool whole) {
+    int done = 0;
+    if (whole) {
+        constexpr int N = Vec<T>::N;
+        for (int q = threadIdx.x; q < n / N; q += TILE_ROWS)
+            reinterpret_cast<uint4 *>(tile)[q] = reinterpret_cast<const uint4 *>(from)[q];
+        done = n / N * N;
+    }
+    for (int e = done + threadIdx.x; e < n; e += TILE_ROWS) tile[e] = from[e];
+}
+template <typename T>
+__device__ __forceinline__ void tile_out(const T *tile, T *to, int n, bool whole) {
+    int done = 0;
+    if (whole) {
+        constexpr int N = Vec<T>::N;
+        for (int q = threadIdx.x; q < n / N; q += TILE_ROWS)
+            reinterpret_cast<uint4 *>(to)[q] = reinterpret_cast<const uint4 *>(tile)[q];
+        done = n / N * N;
+    }
+    for (int e = done + threadIdx.x; e < n; e += TILE_ROWS) to[e] = tile[e];
+}
+
+template <typename T, int OP, bool ENT, int KM>
 __global__ void __launch_bounds__(TILE_ROWS) k_rows_tile(const __grid_constant__ RowsArgs a) {
-    extern __shared__ float tile[];
+    extern __shared__ __align__(16) unsigned char tile_mem[];
     __shared__ double dscratch[33];
-    pdl_wait();
+    T *tile = reinterpret_cast<T *>(tile_mem);
+    early_wait<OP>(a);
     const T *logits = static_cast<const T *>(a.logits);
     T *grad = static_cast<T *>(a.grad);
-    const int K = (int)a.K, pitch = K | 1, tid = threadIdx.x;
+    const int K = (int)a.K, tid = threadIdx.x;
     const float inv_t = 1.0f / a.temperature, c = (float)LOG2E * inv_t;
-    const float w_all = row_weight_all<OP>(a);
+    LateWeight<OP> weight;
     double tot[POL_STATS] = {};
-    const int dr = TILE_ROWS / K, dc = TILE_ROWS - dr * K;  // TILE_ROWS elements on, in rows and columns
-    float *mine = tile + tid * pitch;
+    const bool dense = a.stride == K, dense_out = a.grad_stride == K;
+    const bool whole = reinterpret_cast<uintptr_t>(logits) % 16 == 0, whole_out = reinterpret_cast<uintptr_t>(grad) % 16 == 0;
+    const int words = K * (int)sizeof(T) / 4, g = words & -words;
+    const int turn = K * (int)sizeof(T) % 4 || g == 1 ? 0 : tid / (32 / (g < 32 ? g : 32)) * (4 / (int)sizeof(T)) % K;
+    T *mine = tile + tid * K;
     for (long long i0 = (long long)blockIdx.x * TILE_ROWS; i0 < a.rows; i0 += (long long)gridDim.x * TILE_ROWS) {
         const int n = (int)(a.rows - i0 < TILE_ROWS ? a.rows - i0 : TILE_ROWS);
         const long long i = i0 + tid;
         const bool live = tid < n;
-        const RowIn in = row_open<OP>(a, row_fetch<OP>(a, live ? i : a.rows), w_all);
-        int r = tid / K, k = tid - r * K;
-        for (int e0 = 0; e0 < K; e0 += TILE_BATCH) {  // a thread moves K elements in all
-            float v[TILE_BATCH];
-            int at[TILE_BATCH];
-#pragma unroll
-            for (int e = 0; e < TILE_BATCH; ++e) {
-                at[e] = e0 + e < K && r < n ? r * pitch + k : -1;
-                if (at[e] >= 0) v[e] = Vec<T>::to(logits[(i0 + r) * a.stride + k]);
-                r += dr;
-                k += dc;
-                if (k >= K) {
-                    k -= K;
-                    ++r;
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < TILE_BATCH; ++e)
-                if (at[e] >= 0) tile[at[e]] = v[e];
+        const RowRaw raw = row_fetch<OP>(a, live ? i : a.rows);
+        if (dense) {
+            tile_in(tile, logits + i0 * K, n * K, whole);
+            __syncthreads();
         }
-        __syncthreads();
+        RowIn in = row_open<OP>(a, raw);
+        float x[KM];
+        if (live) {
+            const T *from = dense ? mine : logits + i * a.stride;
+            int at = turn;
+#pragma unroll
+            for (int j = 0; j < KM; ++j) {
+                x[j] = j < K ? Vec<T>::to(from[at]) : -INFINITY;
+                at = at + 1 < K ? at + 1 : 0;
+            }
+        }
         RowSum sum = row_none();
         const bool summed = OP == ROW_GRAD ? row_resum(in) : in.kept;
         if (summed) {
-            for (int j = 0; j < K; ++j) sum.m = fmaxf(sum.m, mine[j]);
+#pragma unroll
+            for (int j = 0; j < KM; ++j) sum.m = fmaxf(sum.m, x[j]);
             const float top = finite_top(sum.m);
-            for (int j = 0; j < K; ++j) {
-                const float d = (mine[j] - top) * c, e = exp2_fast(d);
+#pragma unroll
+            for (int j = 0; j < KM; ++j) {
+                const float d = (x[j] - top) * c, e = exp2_fast(d);
                 sum.s += e;
                 if (ENT && OP != ROW_GRAD) sum.t = fmaf(e, fmaxf(d, D_FLOOR), sum.t);
             }
         }
-        const float x_y = OP != ROW_GRAD && in.kept && in.y < K ? mine[in.y] : NAN;
-        const RowGrad g = row_close<OP, ENT>(a, in, sum, summed, false, x_y, i, live, inv_t, c, tot);
+        const float x_y = OP == ROW_GRAD || !in.kept || in.y >= K ? NAN : Vec<T>::to(dense ? mine[in.y] : logits[i * a.stride + in.y]);
+        weight.set(a, in);
+        const RowGrad r = row_close<OP, ENT>(a, in, sum, summed, false, x_y, i, live, inv_t, c, tot);
         if (OP != ROW_LOGP) {
             if (live) {
-                for (int j = 0; j < K; ++j) mine[j] = one_grad<ENT>(mine[j], g, j == in.y);
-            }
-            __syncthreads();
-            r = tid / K;
-            k = tid - r * K;
-            while (r < n) {
-                grad[(i0 + r) * a.grad_stride + k] = Vec<T>::from(tile[r * pitch + k]);
-                r += dr;
-                k += dc;
-                if (k >= K) {
-                    k -= K;
-                    ++r;
+                T *to = dense_out ? mine : grad + i * a.grad_stride;
+                int at = turn;
+#pragma unroll
+                for (int j = 0; j < KM; ++j) {
+                    if (j < K) to[at] = Vec<T>::from(one_grad<ENT>(x[j], r, at == in.y));
+                    at = at + 1 < K ? at + 1 : 0;
                 }
+            }
+            if (dense_out) {
+                __syncthreads();
+                tile_out(tile, grad + i0 * K, n * K, whole_out);
             }
         }
         __syncthreads();
@@ -1278,17 +1324,22 @@ static int go_ring(const RowsArgs &a, int &grid, cudaStream_t st) {
     return launch_rows(kernel, a.rows, RING_NT, CL, smem, cache, a, grid, st);
 }
 
+template <typename T, int OP, bool ENT, int KM>
+static int go_tile(const RowsArgs &a, int &grid, cudaStream_t st) {
+    static int cache[64];
+    return launch_rows(k_rows_tile<T, OP, ENT, KM>, (a.rows + TILE_ROWS - 1) / TILE_ROWS, TILE_ROWS, 1,
+                       TILE_ROWS * KM * (int)sizeof(T), cache, a, grid, st);
+}
+
 // Which kernel takes rows of K logits: a thread a row up to 32 classes; the
 // registers of 8 or 32 lanes or of a block hold up to 32, 128 and 1024 words;
 // the ring takes longer rows.
 template <typename T, int OP, bool ENT>
 static int run_rows(const RowsArgs &a, int &grid, cudaStream_t st) {
     constexpr int N = Vec<T>::N;
-    if (a.K <= TILE_CLASSES) {
-        static int cache[64];
-        return launch_rows(k_rows_tile<T, OP, ENT>, (a.rows + TILE_ROWS - 1) / TILE_ROWS, TILE_ROWS, 1,
-                           TILE_ROWS * ((int)a.K | 1) * (int)sizeof(float), cache, a, grid, st);
-    }
+    if (a.K <= 8) return go_tile<T, OP, ENT, 8>(a, grid, st);
+    if (a.K <= 16) return go_tile<T, OP, ENT, 16>(a, grid, st);
+    if (a.K <= TILE_CLASSES) return go_tile<T, OP, ENT, TILE_CLASSES>(a, grid, st);
     const long long words = (a.K + 2 * N - 2) / N;  // at most, whatever the alignment
     if (words <= 32) return go_rows<T, OP, ENT, 8, 128, 4>(a, grid, st);
     if (words <= 128) return go_rows<T, OP, ENT, 32, 128, 4>(a, grid, st);
@@ -1402,10 +1453,15 @@ extern "C" int wgb_policy_loss_logits(const void *logits, int32_t dtype, int64_t
     cudaStream_t st = as_stream(stream);
     const PolicyWs w = policy_ws(ws, rows, sequences, seqs);
     const Idx off{seqs ? offsets : nullptr, offset_bytes == 8}, lab{labels, label_bytes == 8};
-    const CountArgs n = count_args(w, mask, lab, rows, off, sequences, rule);
-    static int cache[64];
-    WGB_TRY(launch_all("k_policy_count", k_policy_count<true, GRID_THREADS>, k_policy_count<false, BLOCK_THREADS>,
-                       rows + (by_sequence ? sequences : 0), cache, n, st));
+    CountArgs n = count_args(w, mask, lab, rows, off, sequences, rule);
+    if (seqs) {
+        static int cache[64];
+        WGB_TRY(launch_all("k_policy_count", k_policy_count<true, GRID_THREADS>, k_policy_count<false, BLOCK_THREADS>,
+                           rows + (by_sequence ? sequences : 0), cache, n, st));
+    } else {
+        n.cnt.n_parts = grid_of(rows, KEPT_THREADS * 4, sm_count() * 2);
+        WGB_PDL("k_policy_kept", k_policy_kept, dim3(n.cnt.n_parts), dim3(KEPT_THREADS), 0, st, n);
+    }
     RowsArgs a = {};
     a.logits = logits;
     a.grad = grad;
@@ -1421,7 +1477,7 @@ extern "C" int wgb_policy_loss_logits(const void *logits, int32_t dtype, int64_t
     a.ref = ref_logp;
     a.mask = mask;
     a.rule = rule;
-    a.cnt = w.cnt;
+    a.cnt = n.cnt;
     a.partial = w.partial;
     a.stats = stats;
     int grid = 0;

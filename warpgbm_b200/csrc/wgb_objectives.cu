@@ -620,10 +620,15 @@ struct PolicyCount {
     unsigned *ticket;           // blocks that have written their share of the loss
     unsigned long long *count;  // kept tokens by sequence
     int *ids;                   // sequence of each row (rows of logits), else null
+    unsigned long long *parts;  // where n_parts > 0: blocks' kept tokens, instead of total[0]
+    int n_parts;
 };
-// In fp32: one rounding of a count and one of the quotient.
+// In fp32: one rounding of a count and one of the quotient.  Full warps call it.
 __device__ __forceinline__ float token_weight(const PolicyCount &n) {
-    return n.total[0] ? 1.0f / (float)n.total[0] : 0.0f;
+    unsigned long long kept = 0;
+    for (int i = threadIdx.x & 31; i < n.n_parts; i += 32) kept += n.parts[i];
+    kept = n.n_parts ? warp_sum(kept) : n.total[0];
+    return kept ? 1.0f / (float)kept : 0.0f;
 }
 __device__ __forceinline__ float seq_weight(const PolicyCount &n, long long q) {
     return 1.0f / ((float)n.count[q] * (float)n.total[1]);
@@ -723,9 +728,28 @@ template <bool GRID, int NT>
 __global__ void __launch_bounds__(NT) k_policy_count(const __grid_constant__ CountArgs a) {
     __shared__ double scratch[33];
     pdl_wait();
+    pdl_trigger();
     zero_words(a.cnt.total, a.zero_bytes);
     all_sync<GRID>();
     policy_count<NT>(a, scratch);
+}
+// Counts the kept tokens where there are no sequences: each block its own.
+constexpr int KEPT_THREADS = 512;
+__global__ void __launch_bounds__(KEPT_THREADS) k_policy_kept(const __grid_constant__ CountArgs a) {
+    __shared__ double scratch[33];
+    pdl_wait();
+    pdl_trigger();
+    const Range r = warp_range(a.T);
+    int kept = 0;
+    for (long long t = r.a + (threadIdx.x & 31) * 4; t < r.b; t += STEP) {
+        bool keep[4];
+        quad_mask(a.mask, t, a.T, a.whole_mask, keep);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kept += keep[j] && a.labels.at(t + j) >= 0;
+    }
+    const double k = block_sum((double)kept, scratch);  // whole numbers: exact
+    if (threadIdx.x == 0) a.cnt.parts[blockIdx.x] = (unsigned long long)k;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.cnt.ticket = 0;
 }
 
 struct PolicyTokens {
@@ -1033,7 +1057,10 @@ static PolicyWs policy_ws(void *ws, long long tokens, long long sequences, bool 
     w.partial = reinterpret_cast<double *>(p + at);
     at += round_up256((long long)sm_count() * POL_BLOCKS_PER_SM * POL_STATS * sizeof(double));
     w.cnt.ids = ids ? reinterpret_cast<int *>(p + at) : nullptr;
-    w.bytes = at + (ids ? round_up256(tokens * 4) : 0);
+    at += ids ? round_up256(tokens * 4) : 0;
+    w.cnt.parts = reinterpret_cast<unsigned long long *>(p + at);
+    w.cnt.n_parts = 0;
+    w.bytes = at + round_up256((long long)sm_count() * 2 * sizeof(unsigned long long));
     return w;
 }
 

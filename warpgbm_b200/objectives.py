@@ -21,6 +21,7 @@ sequences are ranges of tokens between neighbouring ``offsets``.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -71,9 +72,12 @@ class PolicyLossLogits(NamedTuple):
 # ---------------------------------------------------------------------------
 
 def _vector(t, name, n, dtypes, dev):
-    """Pointer of a contiguous 1-D CUDA tensor of n values."""
+    """Pointer of a contiguous 1-D tensor of n values (n None: any number) on dev."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype in dtypes and t.get_device() == dev.index and t.dim() == 1 and (n is None or t.shape[0] == n) \
+            and t.is_contiguous():
+        return t.data_ptr()
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
     if t.device != dev:
@@ -150,23 +154,31 @@ def _choice(value, name, table):
     return table[value]
 
 
-class _On:
-    """The device of the call's tensors as the current one; cheaper than
-    torch.cuda.device where it is the current one already."""
-    __slots__ = ("dev", "ctx")
+def _call(name, dev, *args):
+    """The library's `name` on dev's current stream, with dev as the current device."""
+    if torch.cuda.current_device() == dev.index:
+        _lib.call(name, *args, _raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, _raw_stream(dev.index))
 
-    def __init__(self, dev):
-        self.dev, self.ctx = dev, None
 
-    def __enter__(self):
-        if torch.cuda.current_device() != self.dev.index:
-            self.ctx = torch.cuda.device(self.dev)
-            self.ctx.__enter__()
-        return torch.cuda.current_stream().cuda_stream
+@functools.lru_cache(maxsize=64)
+def _preference_ws(sequences, ragged, device_index):
+    return _lib.lib().wgb_preference_ws_bytes(sequences, ragged)
 
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+
+@functools.lru_cache(maxsize=64)
+def _policy_ws(tokens, sequences, rows_of_logits, device_index):
+    return _lib.lib().wgb_policy_ws_bytes(tokens, sequences, rows_of_logits)
+
+
+def _raw_stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same without a Stream object, 3 us less a call
+    _raw_stream = torch._C._cuda_getCurrentRawStream  # noqa: F811
 
 
 # ---------------------------------------------------------------------------
@@ -186,10 +198,9 @@ def label_logprobs(logits, labels, *, temperature=1.0, entropy=False) -> LabelLo
     y = _vector(labels, "labels", n, _INTS, dev)
     temperature = _temperature(temperature)
     out = torch.empty((3 if entropy else 2, n), dtype=torch.float32, device=dev).unbind(0)
-    with _On(dev) as stream:
-        _lib.call("wgb_label_logprobs", logits.data_ptr(), _DTYPES[logits.dtype], n, k, stride, y,
-                  _INDEX_BYTES[labels.dtype], temperature, out[0].data_ptr(), out[1].data_ptr(),
-                  out[2].data_ptr() if entropy else None, stream)
+    _call("wgb_label_logprobs", dev, logits.data_ptr(), _DTYPES[logits.dtype], n, k, stride, y,
+          _INDEX_BYTES[labels.dtype], temperature, out[0].data_ptr(), out[1].data_ptr(),
+          out[2].data_ptr() if entropy else None)
     return LabelLogprobs(out[0], out[1], out[2] if entropy else None)
 
 
@@ -210,9 +221,8 @@ def label_logprobs_grad(logits, labels, lse, grad_logp, *, temperature=1.0, entr
     gh = _optional(grad_entropy, "grad_entropy", n, _F32, dev)
     temperature = _temperature(temperature)
     out, out_stride = _grad_like(logits, stride, out)
-    with _On(dev) as stream:
-        _lib.call("wgb_label_logprobs_grad", logits.data_ptr(), _DTYPES[logits.dtype], n, k, stride, y,
-                  _INDEX_BYTES[labels.dtype], temperature, lse_p, g, h, gh, out.data_ptr(), out_stride, stream)
+    _call("wgb_label_logprobs_grad", dev, logits.data_ptr(), _DTYPES[logits.dtype], n, k, stride, y,
+          _INDEX_BYTES[labels.dtype], temperature, lse_p, g, h, gh, out.data_ptr(), out_stride)
     return out
 
 
@@ -263,16 +273,14 @@ def preference_loss(logp, chosen, rejected, *, ref_logp=None, offsets=None, mask
             raise ValueError("offsets must have one value more than there are sequences")
         off_bytes, sequences = _INDEX_BYTES[offsets.dtype], offsets.shape[0] - 1
     m = _optional(mask, "mask", n, _MASKS, dev)
-    ws_bytes = _lib.lib().wgb_preference_ws_bytes(sequences, off is not None)
+    ws_bytes = _preference_ws(sequences, off is not None, dev.index)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    out = torch.empty(1, dtype=torch.float32, device=dev)
-    grad = torch.empty(n, dtype=torch.float32, device=dev)
-    rewards = torch.empty((2, p), dtype=torch.float32, device=dev).unbind(0)
-    with _On(dev) as stream:
-        _lib.call("wgb_preference_loss", x, ref, n, off, off_bytes, sequences, m, c, r, _INDEX_BYTES[chosen.dtype], p,
-                  w, kind, beta, label_smoothing, bool(average), ws.data_ptr(), ws_bytes, out.data_ptr(),
-                  grad.data_ptr(), rewards[0].data_ptr(), rewards[1].data_ptr(), stream)
-    return PreferenceLoss(out[0], grad, rewards[0], rewards[1])
+    out, grad = logp.new_empty(()), logp.new_empty(n)
+    chosen_reward, rejected_reward = logp.new_empty(p), logp.new_empty(p)
+    _call("wgb_preference_loss", dev, x, ref, n, off, off_bytes, sequences, m, c, r, _INDEX_BYTES[chosen.dtype], p,
+          w, kind, beta, label_smoothing, bool(average), ws.data_ptr(), ws_bytes, out.data_ptr(),
+          grad.data_ptr(), chosen_reward.data_ptr(), rejected_reward.data_ptr())
+    return PreferenceLoss(out, grad, chosen_reward, rejected_reward)
 
 
 # ---------------------------------------------------------------------------
@@ -338,13 +346,11 @@ def policy_loss(logp, old_logp, advantages, *, ref_logp=None, offsets=None, mask
     n = logp.shape[0]
     old, adv, ref, m, off, off_bytes, sequences, adv_by_seq, by_seq, lo, hi, kind, kl_coef = _policy_args(
         n, dev, old_logp, advantages, ref_logp, offsets, mask, clip_low, clip_high, kl_coef, kl, reduction)
-    grad = torch.empty(n, dtype=torch.float32, device=dev)
-    stats = torch.empty(5, dtype=torch.float32, device=dev)
-    with _On(dev) as stream:
-        ws_bytes = _lib.lib().wgb_policy_ws_bytes(n, sequences, 0)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        _lib.call("wgb_policy_loss", x, old, adv, ref, n, m, off, off_bytes, sequences, adv_by_seq, by_seq, lo, hi,
-                  kind, kl_coef, ws.data_ptr(), ws_bytes, stats.data_ptr(), grad.data_ptr(), stream)
+    grad, stats = logp.new_empty(n), logp.new_empty(5)
+    ws_bytes = _policy_ws(n, sequences, 0, dev.index)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    _call("wgb_policy_loss", dev, x, old, adv, ref, n, m, off, off_bytes, sequences, adv_by_seq, by_seq, lo, hi,
+          kind, kl_coef, ws.data_ptr(), ws_bytes, stats.data_ptr(), grad.data_ptr())
     s = stats.unbind(0)
     return PolicyLoss(s[0], grad, s[1], s[2], s[4])
 
@@ -370,12 +376,11 @@ def policy_loss_logits(logits, labels, old_logp, advantages, *, temperature=1.0,
     out, out_stride = _grad_like(logits, stride, out)
     logp = torch.empty(n, dtype=torch.float32, device=dev)
     stats = torch.empty(5, dtype=torch.float32, device=dev)
-    with _On(dev) as stream:
-        ws_bytes = _lib.lib().wgb_policy_ws_bytes(n, sequences, 1)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        _lib.call("wgb_policy_loss_logits", logits.data_ptr(), _DTYPES[logits.dtype], n, k, stride, y,
-                  _INDEX_BYTES[labels.dtype], temperature, old, adv, ref, m, off, off_bytes, sequences, adv_by_seq,
-                  by_seq, lo, hi, kind, kl_coef, entropy_coef, grad_scale, ws.data_ptr(), ws_bytes, stats.data_ptr(),
-                  logp.data_ptr(), out.data_ptr(), out_stride, stream)
+    ws_bytes = _policy_ws(n, sequences, 1, dev.index)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    _call("wgb_policy_loss_logits", dev, logits.data_ptr(), _DTYPES[logits.dtype], n, k, stride, y,
+          _INDEX_BYTES[labels.dtype], temperature, old, adv, ref, m, off, off_bytes, sequences, adv_by_seq,
+          by_seq, lo, hi, kind, kl_coef, entropy_coef, grad_scale, ws.data_ptr(), ws_bytes, stats.data_ptr(),
+          logp.data_ptr(), out.data_ptr(), out_stride)
     s = stats.unbind(0)
     return PolicyLossLogits(s[0], out, logp, s[1], s[2], s[3], s[4])
