@@ -157,8 +157,8 @@ _KERNELS = {
     "wgb_grow_tree": 0, "wgb_bins_feature_major": 1, "wgb_prebinned_ingest": 1,
     "wgb_bin_matrix": 1, "wgb_predict_packed": 1, "wgb_predict_heap": 1, "wgb_quantile_edges": 2, "wgb_quantile_pass": 1, "wgb_quantile_pick": 1,
     "wgb_compute_histogram3": 6, "wgb_compute_histogram3_noalloc": 6,
-    "wgb_label_logprobs": 1, "wgb_label_logprobs_grad": 1, "wgb_preference_loss": 1, "wgb_policy_loss": 1,
-    "wgb_policy_loss_logits": 2,
+    "wgb_label_logprobs": 1, "wgb_label_logprobs_grad": 1, "wgb_preference_loss": 4, "wgb_policy_loss": 3,
+    "wgb_policy_loss_logits": 3,
     "wgb_compute_split": 1, "wgb_custom_cuda_binner": 1, "wgb_predict_forest": 1,
 }
 LAUNCHES = [0]

@@ -1454,14 +1454,7 @@ extern "C" int wgb_policy_loss_logits(const void *logits, int32_t dtype, int64_t
     const PolicyWs w = policy_ws(ws, rows, sequences, seqs);
     const Idx off{seqs ? offsets : nullptr, offset_bytes == 8}, lab{labels, label_bytes == 8};
     CountArgs n = count_args(w, mask, lab, rows, off, sequences, rule);
-    if (seqs) {
-        static int cache[64];
-        WGB_TRY(launch_all("k_policy_count", k_policy_count<true, GRID_THREADS>, k_policy_count<false, BLOCK_THREADS>,
-                           rows + (by_sequence ? sequences : 0), cache, n, st));
-    } else {
-        n.cnt.n_parts = grid_of(rows, KEPT_THREADS * 4, sm_count() * 2);
-        WGB_PDL("k_policy_kept", k_policy_kept, dim3(n.cnt.n_parts), dim3(KEPT_THREADS), 0, st, n);
-    }
+    WGB_TRY(launch_counts(n, st));
     RowsArgs a = {};
     a.logits = logits;
     a.grad = grad;

@@ -3,18 +3,18 @@
 // include/warpgbm_b200.h; the calls that take rows of logits are in
 // wgb_logits.cu).
 //
-// A call is one launch.  What comes first has to be complete before the next
-// part can start (kept tokens are counted before their gradient is scaled, a
-// sequence is summed before its pairs are compared), so the parts are separated
-// by a barrier: of a cooperative grid, or of the one block that small calls
-// take, which then costs a launch and a few microseconds.
+// A call has parts that each need the one before complete: kept tokens are
+// counted before their gradient is scaled, a sequence is summed before its pairs
+// are compared.  Small calls run them in one block with barriers between, which
+// costs one launch.  Others launch a kernel for each part, the next one started
+// early (pdl_trigger) so that its blocks are in place when the part before ends;
+// barriers of a cooperative grid took longer than that (22 us with the parts'
+// work left out, against about 2 us a part).
 //
 // Sums over the tokens of a sequence and over the pairs of a sequence are
 // exact: a partial sum formed in a fixed order is added to a 128-bit
 // fixed-point number with integer atomics (Sums), so no result depends on the
 // order of the atomics.
-#include <cooperative_groups.h>
-
 #include <type_traits>
 
 namespace wgb {
@@ -28,11 +28,10 @@ struct Idx {
     }
 };
 
-// Everything before is done, and visible, for the whole launch.
-template <bool GRID>
-__device__ __forceinline__ void all_sync() {
-    if constexpr (GRID) cooperative_groups::this_grid().sync();
-    else __syncthreads();
+// A kernel of one part: after the part before it, and the next may be put in place.
+__device__ __forceinline__ void part_begin() {
+    pdl_wait();
+    pdl_trigger();
 }
 
 __device__ __forceinline__ double block_sum(double v, double *scratch /* >= 33 */) {
@@ -62,6 +61,8 @@ __device__ __forceinline__ bool last_of_grid(unsigned *ticket) {
     }
     return __shfl_sync(0xffffffffu, mine, 0) == gridDim.x - 1;
 }
+
+constexpr int GRID_THREADS = 256, BLOCK_THREADS = 1024;
 
 // ------------------------------------------------------- exact totals --
 // Sums of real numbers as 128-bit two's complement numbers of 2^-64ths, so that
@@ -183,31 +184,42 @@ __device__ __forceinline__ long long upper_bound_one(const Idx &off, long long l
 
 // The warp's place among the launch's warps, and its range of tokens.
 __device__ __forceinline__ long long warp_index() { return ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; }
-__device__ __forceinline__ long long warp_count() { return ((long long)gridDim.x * blockDim.x) >> 5; }
 struct Range {
     long long a, b;
 };
-__device__ __forceinline__ Range warp_range(long long T) {
-    const long long steps = (T + STEP - 1) / STEP, n = warp_count(), i = warp_index();
-    const long long each = steps / n, more = steps % n;
-    const long long first = i * each + (i < more ? i : more);
-    const long long a = first * STEP, b = (first + each + (i < more)) * STEP;
-    return Range{a < T ? a : T, b < T ? b : T};
+// How a launch's warps share the tokens' steps: `each` of them, the first `more`
+// warps one more (worked out by the host: 64-bit divisions are slow here).
+struct Cut {
+    long long T, each, more;
+    __device__ __forceinline__ Range range() const {
+        const long long i = warp_index();
+        const long long first = i * each + (i < more ? i : more);
+        const long long a = first * STEP, b = (first + each + (i < more)) * STEP;
+        return Range{a < T ? a : T, b < T ? b : T};
+    }
+};
+inline Cut cut_of(long long T, long long warps) {
+    const long long steps = (T + STEP - 1) / STEP;
+    return Cut{T, steps / warps, steps % warps};
 }
 
 // Where a warp is: sequence q (-1 before the first, S after the last) holds the
-// tokens up to `end`.  All lanes have the same.
+// tokens up to `end`, the one after it those up to `end2`, loaded ahead.  All
+// lanes have the same.
 struct Place {
-    long long q, end;
+    long long q, end, end2;
+    __device__ __forceinline__ void ahead(const Idx &off, long long S) { end2 = q + 2 <= S ? off.at(q + 2) : LLONG_MAX; }
     __device__ __forceinline__ void find(const Idx &off, long long S, long long lo, long long t) {
         q = upper_bound_warp(off, lo, S + 1, t) - 1;
         end = q < S ? off.at(q + 1) : LLONG_MAX;
+        ahead(off, S);
     }
     // To the sequence of token t = end.
     __device__ __forceinline__ void next(const Idx &off, long long S, long long t) {
-        if (q + 2 <= S && off.at(q + 2) > t) {
+        if (q + 2 <= S && end2 > t) {
             ++q;
-            end = off.at(q + 1);
+            end = end2;
+            ahead(off, S);
         } else {
             find(off, S, q + 1 < S + 1 ? q + 1 : S + 1, t);
         }
@@ -218,7 +230,7 @@ struct Place {
 // look for their own.
 constexpr int MANY = 6;
 __device__ __forceinline__ bool many_seqs(const Idx &off, long long S, const Place &at, long long t1) {
-    return at.end < t1 && at.q + MANY <= S && off.at(at.q + MANY) < t1;
+    return at.end2 < t1 && at.q + MANY <= S && off.at(at.q + MANY) < t1;
 }
 // Sequences of the four tokens from t on (-1: none), at.q .. last being those of
 // the step.
@@ -293,29 +305,45 @@ __device__ __forceinline__ void warp_by_seq(long long q, double v, int n, F add)
 
 // Sums of a warp's range by sequence: fetch(t, keep, v) gives the four tokens
 // from t on whether they are kept and their values; add(q, v, n), called by one
-// lane, takes what the range has of sequence q.
-template <typename FETCH, typename ADD>
-__device__ __forceinline__ void range_by_seq(const Idx &off, long long S, const Range &r, FETCH fetch, ADD add) {
+// lane, takes what the range has of sequence q.  `start` gets the range's first
+// place, for the parts to come.
+template <bool VALUES, typename FETCH, typename ADD>
+__device__ __forceinline__ void range_by_seq(const Idx &off, long long S, const Range &r, Place *start, FETCH fetch, ADD add) {
     if (r.a >= r.b) return;
     const int lane = threadIdx.x & 31;
     Place at;
     at.find(off, S, 0, r.a);
+    if (lane == 0) start[warp_index()] = at;
     double sum = 0.0;  // of the sequence that the warp is in
     int count = 0;
     auto flush = [&]() {
-        const double v = warp_sum(sum);
+        const double v = VALUES ? warp_sum(sum) : 0.0;
         const int n = warp_sum(count);
         if (lane == 0 && n && at.valid(S)) add(at.q, v, n);
         sum = 0.0;
         count = 0;
     };
+    bool more[4];
+    float ahead[4];
+    fetch(r.a + lane * 4, more, ahead);  // says no past the last token, where a range may end
     for (long long t0 = r.a; t0 < r.b; t0 += STEP) {
         const long long t1 = t0 + STEP < r.b ? t0 + STEP : r.b, t = t0 + lane * 4;
         bool keep[4];
         float v[4];
-        fetch(t, keep, v);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) keep[j] = keep[j] && t + j < t1;
+        for (int j = 0; j < 4; ++j) {
+            keep[j] = more[j];
+            v[j] = ahead[j];
+        }
+        if (t1 < r.b) fetch(t + STEP, more, ahead);
+        if (at.end >= t1 && at.end > t0) {  // one sequence
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (VALUES) sum += keep[j] ? (double)v[j] : 0.0;
+                count += keep[j];
+            }
+            continue;
+        }
         if (many_seqs(off, S, at, t1)) {
             flush();
             const long long first = at.q;
@@ -323,20 +351,21 @@ __device__ __forceinline__ void range_by_seq(const Idx &off, long long S, const 
             long long q[4];
             quad_seqs(off, S, first, at.q, t, q);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) warp_by_seq(q[j], keep[j] ? (double)v[j] : 0.0, keep[j], add);
+            for (int j = 0; j < 4; ++j) warp_by_seq(q[j], VALUES && keep[j] ? (double)v[j] : 0.0, keep[j], add);
             continue;
         }
-        for (long long from = t0; from < t1;) {
-            if (at.end <= from) {
+        const int n = (int)(t1 - t0);
+        for (int from = 0; from < n;) {
+            if (at.end <= t0 + from) {
                 flush();
-                at.next(off, S, from);
-                if (at.end <= from) break;  // offsets that do not rise
+                at.next(off, S, t0 + from);
+                if (at.end <= t0 + from) break;  // offsets that do not rise
             }
-            const long long to = at.end < t1 ? at.end : t1;
+            const int to = at.end < t1 ? (int)(at.end - t0) : n;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (keep[j] && t + j >= from && t + j < to) {
-                    sum += (double)v[j];
+                if (keep[j] && lane * 4 + j >= from && lane * 4 + j < to) {
+                    if (VALUES) sum += (double)v[j];
                     ++count;
                 }
             from = to;
@@ -398,7 +427,10 @@ struct PrefArgs {
     Sums grads, scores;         // by sequence: gradient, sum of log ratios (ragged)
     unsigned long long *count;  // kept tokens by sequence (ragged)
     float *diff;                // logp - ref by row (not ragged, with a reference)
+    Place *places;              // where each warp's range of tokens starts (ragged)
     bool whole, whole_mask;     // arrays on 16-byte (mask: 4-byte) boundaries
+    int n_top, n_partial;       // blocks that gave a weight, a share of the loss
+    Cut cut;
 };
 
 // Score of sequence q: its sum (or mean) of log ratios; NaN out of range.
@@ -417,14 +449,24 @@ __device__ __forceinline__ float warp_max(float v) {
 constexpr int PAIR_EACH = 4;  // pairs of a thread under way together: they are gathers, and wait for memory
 
 // Bytes: 13 a token read and 4 written, 16 a pair and the gathers of its
-// scores.  Time goes to the barriers and, with many pairs, to the atomics of
-// their gradients: two a pair, which a bound on their terms allows for (the
-// square loss has none and takes up to four).
-template <bool GRID, int NT>
-__global__ void __launch_bounds__(NT) k_preference(const __grid_constant__ PrefArgs a) {
-    __shared__ double scratch[33];
+// scores.  With many pairs time goes to the gathers and to the atomics of their
+// gradients: two a pair, which a bound on their terms allows for (the square loss
+// has none and takes up to four).
+// The bound on a pair's gradient, from the blocks' largest weights.
+__device__ __forceinline__ GridSums pref_grid_sums(const PrefArgs &a) {
+    float bound = a.rule.beta;
+    if (a.rule.kind != 2 && a.weight) {
+        float top = 0.0f;
+        for (int i = threadIdx.x & 31; i < a.n_top; i += 32) top = fmaxf(top, a.top[i]);
+        bound *= warp_max(top);
+    }
+    return GridSums(a.grads, bound, 2 * a.P + 1);
+}
+
+// What starts as zeros; differences by row; the largest weight.
+template <int NT>
+__device__ __forceinline__ void pref_start(const PrefArgs &a) {
     __shared__ float tops[33];
-    pdl_wait();
     const long long me = (long long)blockIdx.x * NT + threadIdx.x, all = (long long)gridDim.x * NT;
     zero_words(a.zeros, a.zero_bytes);
     if (!a.off.p && a.ref)
@@ -444,32 +486,31 @@ __global__ void __launch_bounds__(NT) k_preference(const __grid_constant__ PrefA
             if (threadIdx.x == 0) a.top[blockIdx.x] = top;
         }
     }
-    all_sync<GRID>();
-    float bound = a.rule.beta;
-    if (bounded && a.weight) {
-        float top = 0.0f;
-        for (int i = threadIdx.x & 31; i < (int)gridDim.x; i += 32) top = fmaxf(top, a.top[i]);
-        bound *= warp_max(top);
-    }
-    const GridSums grid_sums(a.grads, bound, 2 * a.P + 1);
-    if (a.off.p) {
-        range_by_seq(a.off, a.S, warp_range(a.T),
-            [&](long long t, bool (&keep)[4], float (&v)[4]) {
-                quad_mask(a.mask, t, a.T, a.whole_mask, keep);
-                quad_load(a.logp, t, a.T, a.whole, 0.0f, v);
-                if (a.ref) {
-                    float r[4];
-                    quad_load(a.ref, t, a.T, a.whole, 0.0f, r);
+}
+// Sequence sums of logp - ref over the kept tokens.
+__device__ __forceinline__ void pref_sums(const PrefArgs &a) {
+    range_by_seq<true>(a.off, a.S, a.cut.range(), a.places,
+        [&](long long t, bool (&keep)[4], float (&v)[4]) {
+            quad_mask(a.mask, t, a.T, a.whole_mask, keep);
+            quad_load(a.logp, t, a.T, a.whole, 0.0f, v);
+            if (a.ref) {
+                float r[4];
+                quad_load(a.ref, t, a.T, a.whole, 0.0f, r);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] -= r[j];
-                }
-            },
-            [&](long long q, double v, int n) {
-                a.scores.add(q, v);
-                atomicAdd(a.count + q, (unsigned long long)n);
-            });
-        all_sync<GRID>();
-    }
+                for (int j = 0; j < 4; ++j) v[j] -= r[j];
+            }
+        },
+        [&](long long q, double v, int n) {
+            a.scores.add(q, v);
+            atomicAdd(a.count + q, (unsigned long long)n);
+        });
+}
+// Losses of the pairs, and their gradients to the sequences.
+template <int NT>
+__device__ __forceinline__ void pref_pairs(const PrefArgs &a, double *scratch) {
+    const long long me = (long long)blockIdx.x * NT + threadIdx.x, all = (long long)gridDim.x * NT;
+    const bool bounded = a.rule.kind != 2;
+    const GridSums grid_sums = pref_grid_sums(a);
     double total = 0.0;
     for (long long p0 = me; p0 < a.P; p0 += all * PAIR_EACH) {
         long long c[PAIR_EACH], r[PAIR_EACH];
@@ -509,11 +550,16 @@ __global__ void __launch_bounds__(NT) k_preference(const __grid_constant__ PrefA
     }
     total = block_sum(total, scratch);
     if (threadIdx.x == 0) a.partial[blockIdx.x] = total;
-    all_sync<GRID>();
+}
+// The loss, and the gradient of every token: its sequence's, where it is kept.
+template <int NT>
+__device__ __forceinline__ void pref_grad(const PrefArgs &a, double *scratch) {
+    const bool bounded = a.rule.kind != 2;
+    const GridSums grid_sums = pref_grid_sums(a);
     const double inv = a.P ? 1.0 / (double)a.P : 0.0;
     if (blockIdx.x == 0) {
         double v = 0.0;
-        for (int i = threadIdx.x; i < (int)gridDim.x; i += NT) v += a.partial[i];
+        for (int i = threadIdx.x; i < a.n_partial; i += NT) v += a.partial[i];
         v = block_sum(v, scratch);
         if (threadIdx.x == 0) *a.loss = (float)(v * inv);
     }
@@ -521,7 +567,7 @@ __global__ void __launch_bounds__(NT) k_preference(const __grid_constant__ PrefA
         const double v = (bounded ? grid_sums.value(q) : a.grads.value(q)) * inv;
         return (float)(a.rule.average && a.count[q] ? v / (double)a.count[q] : v);
     };
-    const Range range = warp_range(a.T);
+    const Range range = a.cut.range();
     const int lane = threadIdx.x & 31;
     if (!a.off.p) {
         for (long long t = range.a + lane * 4; t < range.b; t += STEP) {
@@ -533,8 +579,7 @@ __global__ void __launch_bounds__(NT) k_preference(const __grid_constant__ PrefA
         return;
     }
     if (range.a >= range.b) return;
-    Place at;
-    at.find(a.off, a.S, 0, range.a);
+    Place at = a.places[warp_index()];
     float of = at.valid(a.S) ? grad_of(at.q) : 0.0f;
     for (long long t0 = range.a; t0 < range.b; t0 += STEP) {
         const long long t1 = t0 + STEP < range.b ? t0 + STEP : range.b, t = t0 + lane * 4;
@@ -568,7 +613,37 @@ __global__ void __launch_bounds__(NT) k_preference(const __grid_constant__ PrefA
     }
 }
 
+template <int PART>
+__global__ void __launch_bounds__(GRID_THREADS) k_pref_part(const __grid_constant__ PrefArgs a) {
+    __shared__ double scratch[33];
+    part_begin();
+    if (PART == 0) pref_start<GRID_THREADS>(a);
+    if (PART == 1) pref_sums(a);
+    if (PART == 2) pref_pairs<GRID_THREADS>(a, scratch);
+    if (PART == 3) pref_grad<GRID_THREADS>(a, scratch);
+}
+__global__ void __launch_bounds__(BLOCK_THREADS) k_pref_block(const __grid_constant__ PrefArgs a) {
+    __shared__ double scratch[33];
+    part_begin();
+    pref_start<BLOCK_THREADS>(a);
+    __syncthreads();
+    if (a.off.p) {
+        pref_sums(a);
+        __syncthreads();
+    }
+    pref_pairs<BLOCK_THREADS>(a, scratch);
+    __syncthreads();
+    pref_grad<BLOCK_THREADS>(a, scratch);
+}
+
 // ------------------------------------------------------------- policy --
+// e^x as 2^(x log2 e): relative error 2^-22 and 2^-24 |x|.
+__device__ __forceinline__ float exp_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504088896340736f));
+    return r;
+}
+
 struct PolicyRule {
     float clip_hi, clip_lo, log_hi, log_lo;  // 1 + high, 1 - low and their logarithms
     float kl_coef, ent_coef, grad_scale;
@@ -583,7 +658,7 @@ __device__ __forceinline__ PolicyTerm policy_term(const PolicyRule &r, float log
     PolicyTerm p;
     const float u = logp - old;
     const bool hi = adv > 0 && u > r.log_hi, lo = adv < 0 && u < r.log_lo;
-    const float ratio = expf(u);
+    const float ratio = exp_fast(u);
     p.pg = -adv * (hi ? r.clip_hi : lo ? r.clip_lo : ratio);
     p.dpg = hi || lo ? 0.0f : -adv * ratio;
     p.cut = hi || lo ? 1.0f : 0.0f;
@@ -597,18 +672,14 @@ __device__ __forceinline__ PolicyTerm policy_term(const PolicyRule &r, float log
             p.kl = 0.5f * d * d;
             p.dkl = -d;
         } else {
-            // e^d - 1 - d loses its digits near zero: Taylor's series there
-            // (the term left out is below 2^-24 of the sum)
-            if (fabsf(d) < 0.35f) {
-                p.kl = 0.5f * d * d *
-                       fmaf(d * (1.0f / 3), fmaf(d * 0.25f, fmaf(d * 0.2f, fmaf(d * (1.0f / 6),
-                       fmaf(d * (1.0f / 7), fmaf(d, 0.125f, 1.0f), 1.0f), 1.0f), 1.0f), 1.0f), 1.0f);
-                p.dkl = -(p.kl + d);
-            } else {
-                const float e = expf(d) - 1.0f;
-                p.kl = e - d;
-                p.dkl = -e;
-            }
+            // e^d - 1 - d loses its digits near zero: Taylor's series there (the
+            // term left out is below 2^-24 of the sum)
+            const float near = 0.5f * d * d *
+                               fmaf(d * (1.0f / 3), fmaf(d * 0.25f, fmaf(d * 0.2f, fmaf(d * (1.0f / 6),
+                               fmaf(d * (1.0f / 7), fmaf(d, 0.125f, 1.0f), 1.0f), 1.0f), 1.0f), 1.0f), 1.0f);
+            const float e = exp_fast(d) - 1.0f;
+            p.kl = fabsf(d) < 0.35f ? near : e - d;
+            p.dkl = fabsf(d) < 0.35f ? -(near + d) : -e;
         }
     }
     return p;
@@ -620,6 +691,7 @@ struct PolicyCount {
     unsigned *ticket;           // blocks that have written their share of the loss
     unsigned long long *count;  // kept tokens by sequence
     int *ids;                   // sequence of each row (rows of logits), else null
+    Place *places;              // where each warp's range of tokens starts
     unsigned long long *parts;  // where n_parts > 0: blocks' kept tokens, instead of total[0]
     int n_parts;
 };
@@ -673,15 +745,15 @@ struct CountArgs {
     bool by_sequence, whole_mask;
     PolicyCount cnt;
     long long zero_bytes;  // from cnt.total on
+    Cut cut;
 };
 
 // Counts the kept tokens, in all and by sequence; with ids also writes each
 // token's sequence.  A token is kept where mask and label say so and, with
 // offsets, a sequence holds it.
-template <int NT>
 __device__ __forceinline__ void policy_count(const CountArgs &a, double *scratch) {
     long long kept = 0, full = 0;
-    const Range r = warp_range(a.T);
+    const Range r = a.cut.range();
     auto fetch = [&](long long t, bool (&keep)[4], float (&v)[4]) {
         quad_mask(a.mask, t, a.T, a.whole_mask, keep);
 #pragma unroll
@@ -691,15 +763,15 @@ __device__ __forceinline__ void policy_count(const CountArgs &a, double *scratch
         }
     };
     if (a.off.p) {
-        range_by_seq(a.off, a.S, r, fetch, [&](long long q, double, int n) {
+        range_by_seq<false>(a.off, a.S, r, a.cnt.places, fetch, [&](long long q, double, int n) {
             if (a.by_sequence) full += atomicAdd(a.cnt.count + q, (unsigned long long)n) == 0;
             kept += n;
         });
         if (a.cnt.ids && r.a < r.b) {
+            __syncwarp();
+            const long long first = a.cnt.places[warp_index()].q;
             Place at;
-            at.find(a.off, a.S, 0, r.a);
-            const long long first = at.q;
-            at.find(a.off, a.S, 0, r.b - 1);
+            at.find(a.off, a.S, first + 1, r.b - 1);
             for (long long t = r.a + (threadIdx.x & 31) * 4; t < r.b; t += STEP) {
                 long long q[4];
                 quad_seqs(a.off, a.S, first, at.q, t, q);
@@ -724,28 +796,34 @@ __device__ __forceinline__ void policy_count(const CountArgs &a, double *scratch
         if (f > 0) atomicAdd(a.cnt.total + 1, (unsigned long long)f);
     }
 }
-template <bool GRID, int NT>
-__global__ void __launch_bounds__(NT) k_policy_count(const __grid_constant__ CountArgs a) {
-    __shared__ double scratch[33];
-    pdl_wait();
-    pdl_trigger();
+__global__ void __launch_bounds__(GRID_THREADS) k_policy_zero(const __grid_constant__ CountArgs a) {
+    part_begin();
     zero_words(a.cnt.total, a.zero_bytes);
-    all_sync<GRID>();
-    policy_count<NT>(a, scratch);
+}
+__global__ void __launch_bounds__(GRID_THREADS) k_policy_count(const __grid_constant__ CountArgs a) {
+    __shared__ double scratch[33];
+    part_begin();
+    policy_count(a, scratch);
+}
+__global__ void __launch_bounds__(BLOCK_THREADS) k_policy_count_block(const __grid_constant__ CountArgs a) {
+    __shared__ double scratch[33];
+    part_begin();
+    zero_words(a.cnt.total, a.zero_bytes);
+    __syncthreads();
+    policy_count(a, scratch);
 }
 // Counts the kept tokens where there are no sequences: each block its own.
 constexpr int KEPT_THREADS = 512;
 __global__ void __launch_bounds__(KEPT_THREADS) k_policy_kept(const __grid_constant__ CountArgs a) {
     __shared__ double scratch[33];
-    pdl_wait();
-    pdl_trigger();
-    const Range r = warp_range(a.T);
+    part_begin();
+    const Range r = a.cut.range();
     int kept = 0;
     for (long long t = r.a + (threadIdx.x & 31) * 4; t < r.b; t += STEP) {
         bool keep[4];
         quad_mask(a.mask, t, a.T, a.whole_mask, keep);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) kept += keep[j] && a.labels.at(t + j) >= 0;
+        for (int j = 0; j < 4; ++j) kept += keep[j] && (!a.labels.p || a.labels.at(t + j) >= 0);
     }
     const double k = block_sum((double)kept, scratch);  // whole numbers: exact
     if (threadIdx.x == 0) a.cnt.parts[blockIdx.x] = (unsigned long long)k;
@@ -761,43 +839,69 @@ struct PolicyTokens {
     bool whole;
 };
 // Bytes: 17 a token read (and its mask byte twice), 4 written.
-template <bool GRID, int NT>
-__global__ void __launch_bounds__(NT) k_policy_tokens(const __grid_constant__ PolicyTokens a) {
-    __shared__ double scratch[33];
-    pdl_wait();
+__device__ __forceinline__ void policy_tokens(const PolicyTokens &a, double *scratch) {
     const CountArgs &n = a.count;
-    zero_words(n.cnt.total, n.zero_bytes);
-    all_sync<GRID>();
-    policy_count<NT>(n, scratch);
-    all_sync<GRID>();
     double sum[POL_STATS] = {};
     const PolicyRule &rule = a.rule;
     const float w_all = rule.by_sequence ? 0.0f : token_weight(n.cnt);
-    const Range r = warp_range(n.T);
+    const Range r = n.cut.range();
     const int lane = threadIdx.x & 31;
-    Place at{0, LLONG_MAX};
+    // a step's values are loaded while the step before is worked on
+    struct Quad {
+        bool keep[4];
+        float x[4], old[4], adv[4], ref[4];
+    } more;
+    auto fetch = [&](long long t) {
+        quad_mask(n.mask, t, n.T, n.whole_mask, more.keep);
+        quad_load(a.logp, t, n.T, a.whole, 0.0f, more.x);
+        quad_load(a.old, t, n.T, a.whole, 0.0f, more.old);
+        if (!rule.adv_by_sequence) quad_load(a.adv, t, n.T, a.whole, 0.0f, more.adv);
+        if (rule.kl_kind) quad_load(a.ref, t, n.T, a.whole, 0.0f, more.ref);
+    };
+#pragma unroll
+    for (int j = 0; j < 4; ++j) more.adv[j] = more.ref[j] = 0.0f;
+    if (r.a < r.b) fetch(r.a + lane * 4);
+    Place at{0, LLONG_MAX, LLONG_MAX};
     float wt = w_all, av = 0.0f;  // of the sequence that the warp is in
     bool in = true;
     auto weight_of = [&](long long q) { return rule.by_sequence && n.cnt.count[q] ? seq_weight(n.cnt, q) : w_all; };
+    // The next sequence's count and advantage are loaded ahead.
+    long long held_q = -2;
+    unsigned long long held_n = 0;
+    float held_a = 0.0f;
+    const float full = (float)n.cnt.total[1];
     auto enter = [&]() {
         in = at.valid(n.S);
-        wt = in ? weight_of(at.q) : 0.0f;
-        av = in && rule.adv_by_sequence ? a.adv[at.q] : 0.0f;
+        if (in && at.q != held_q) {
+            if (rule.by_sequence) held_n = n.cnt.count[at.q];
+            if (rule.adv_by_sequence) held_a = a.adv[at.q];
+        }
+        wt = !in ? 0.0f : rule.by_sequence && held_n ? 1.0f / ((float)held_n * full) : w_all;
+        av = in ? held_a : 0.0f;
+        held_q = at.q + 1;
+        if (held_q >= 0 && held_q < n.S) {
+            if (rule.by_sequence) held_n = n.cnt.count[held_q];
+            if (rule.adv_by_sequence) held_a = a.adv[held_q];
+        }
     };
     if (n.off.p && r.a < r.b) {
-        at.find(n.off, n.S, 0, r.a);
+        at = n.cnt.places[warp_index()];
         enter();
     }
     for (long long t0 = r.a; t0 < r.b; t0 += STEP) {
         const long long t1 = t0 + STEP < r.b ? t0 + STEP : r.b, t = t0 + lane * 4;
         bool keep[4];
-        float x[4], old[4], adv[4] = {av, av, av, av}, w[4] = {wt, wt, wt, wt}, ref[4] = {0.0f, 0.0f, 0.0f, 0.0f}, g[4];
-        quad_mask(n.mask, t, n.T, n.whole_mask, keep);
-        quad_load(a.logp, t, n.T, a.whole, 0.0f, x);
-        quad_load(a.old, t, n.T, a.whole, 0.0f, old);
-        if (!rule.adv_by_sequence) quad_load(a.adv, t, n.T, a.whole, 0.0f, adv);
-        if (rule.kl_kind) quad_load(a.ref, t, n.T, a.whole, 0.0f, ref);
-        if (at.end >= t1) {  // one sequence
+        float x[4], old[4], adv[4], w[4] = {wt, wt, wt, wt}, ref[4], g[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            keep[j] = more.keep[j];
+            x[j] = more.x[j];
+            old[j] = more.old[j];
+            adv[j] = rule.adv_by_sequence ? av : more.adv[j];
+            ref[j] = more.ref[j];
+        }
+        if (t1 < r.b) fetch(t + STEP);
+        if (at.end >= t1 && at.end > t0) {  // one sequence
 #pragma unroll
             for (int j = 0; j < 4; ++j) keep[j] = keep[j] && in;
         } else if (many_seqs(n.off, n.S, at, t1)) {
@@ -852,6 +956,20 @@ __global__ void __launch_bounds__(NT) k_policy_tokens(const __grid_constant__ Po
         quad_store(a.grad, t, n.T, a.whole, g);
     }
     policy_end_block(sum, rule, n.cnt.ticket, a.partial, a.stats, scratch);
+}
+__global__ void __launch_bounds__(GRID_THREADS, 3) k_policy_tokens(const __grid_constant__ PolicyTokens a) {
+    __shared__ double scratch[33];
+    part_begin();
+    policy_tokens(a, scratch);
+}
+__global__ void __launch_bounds__(BLOCK_THREADS) k_policy_tokens_block(const __grid_constant__ PolicyTokens a) {
+    __shared__ double scratch[33];
+    part_begin();
+    zero_words(a.count.cnt.total, a.count.zero_bytes);
+    __syncthreads();
+    policy_count(a.count, scratch);
+    __syncthreads();
+    policy_tokens(a, scratch);
 }
 
 // ---------------------------------------------------------------- host --
@@ -911,37 +1029,16 @@ static int check_index(const char *name, int bytes) {
     } while (0)
 
 
-// Launches `kernel<true, 256>` over all SMs as a cooperative grid, or
-// `kernel<false, 1024>` as one block for at most ONE_BLOCK tokens' worth of work,
-// which a block does in the time of a grid's barriers.
+// One block for at most this many tokens' worth of work: it does them in the time
+// of the other form's launches.
 constexpr long long ONE_BLOCK = 16384;
-constexpr int GRID_THREADS = 256, BLOCK_THREADS = 1024;
 constexpr int MAX_BLOCKS_PER_SM = 8;
-template <typename A>
-static int launch_all(const char *name, void (*grid_kernel)(A), void (*block_kernel)(A), long long work, int (&cache)[64],
-                      const A &args, cudaStream_t st) {
-    if (work <= ONE_BLOCK) {
-        WGB_PDL(name, block_kernel, dim3(1), dim3(BLOCK_THREADS), 0, st, args);
-        return WGB_OK;
-    }
-    long long most = resident(grid_kernel, GRID_THREADS, 1, 0, cache);
-    if (most > (long long)sm_count() * MAX_BLOCKS_PER_SM) most = (long long)sm_count() * MAX_BLOCKS_PER_SM;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid_of(work, GRID_THREADS * 4, (int)most));
-    cfg.blockDim = dim3(GRID_THREADS);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeCooperative;
-    at[0].val.cooperative = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, grid_kernel, args);
-    if (e != cudaSuccess) {
-        set_error("launch of %s failed: %s", name, cudaGetErrorString(e));
-        return WGB_ERR_CUDA;
-    }
-    return WGB_OK;
-}
+// Blocks of a part that goes over `items`, `each` of them to a block at least.
+static int part_grid(long long items, int each) { return grid_of(items, each, sm_count() * MAX_BLOCKS_PER_SM); }
+// Blocks of a part whose warps walk ranges of tokens: as many as are resident
+// together, since a warp's start costs as much as several steps.
+static int walk_grid(long long tokens) { return grid_of(tokens, GRID_THREADS / 32 * STEP, sm_count() * 3); }
+static long long places_bytes() { return (long long)sm_count() * MAX_BLOCKS_PER_SM * (GRID_THREADS / 32) * sizeof(Place); }
 static bool on16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 static bool on4(const void *p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 
@@ -957,6 +1054,7 @@ struct PrefWs {
     Sums grads, scores;
     unsigned long long *count;
     float *top, *diff;
+    Place *places;
 };
 static PrefWs pref_ws(void *ws, long long sequences, bool ragged) {
     PrefWs w;
@@ -975,7 +1073,8 @@ static PrefWs pref_ws(void *ws, long long sequences, bool ragged) {
     if (ragged) at += (sequences + 1) / 2 * 16;
     w.zero_bytes = at - from;
     w.diff = reinterpret_cast<float *>(p + at);
-    if (!ragged) at += 4 * sequences;
+    w.places = reinterpret_cast<Place *>(p + at);
+    at += ragged ? places_bytes() : 4 * sequences;
     w.bytes = round_up256(at);
     return w;
 }
@@ -1031,12 +1130,27 @@ extern "C" int wgb_preference_loss(const float *logp, const float *ref_logp, int
     a.count = w.count;
     a.top = w.top;
     a.diff = w.diff;
+    a.places = w.places;
     a.whole = on16(logp) && on16(ref_logp) && on16(grad_logp);
     a.whole_mask = on4(mask);
-    static int cache[64];
+    cudaStream_t st = as_stream(stream);
+    const dim3 nt(GRID_THREADS);
     // a pair costs about as much as four tokens, a sequence as two
-    return launch_all("k_preference", k_preference<true, GRID_THREADS>, k_preference<false, BLOCK_THREADS>,
-                      tokens + 4 * pairs + 2 * sequences, cache, a, as_stream(stream));
+    if (tokens + 4 * pairs + 2 * sequences <= ONE_BLOCK) {
+        a.n_top = a.n_partial = 1;
+        a.cut = cut_of(tokens, BLOCK_THREADS / 32);
+        WGB_PDL("k_pref_block", k_pref_block, dim3(1), dim3(BLOCK_THREADS), 0, st, a);
+        return WGB_OK;
+    }
+    const int start = part_grid(tokens + pairs + 2 * sequences, 1024), tok = offsets ? walk_grid(tokens) : part_grid(tokens, 1024);
+    a.cut = cut_of(tokens, tok * (GRID_THREADS / 32));
+    a.n_top = start;
+    a.n_partial = part_grid(pairs, GRID_THREADS);
+    WGB_PDL("k_pref_part", k_pref_part<0>, dim3(start), nt, 0, st, a);
+    if (offsets) WGB_PDL("k_pref_part", k_pref_part<1>, dim3(tok), nt, 0, st, a);
+    WGB_PDL("k_pref_part", k_pref_part<2>, dim3(a.n_partial), nt, 0, st, a);
+    WGB_PDL("k_pref_part", k_pref_part<3>, dim3(tok), nt, 0, st, a);
+    return WGB_OK;
 }
 
 namespace wgb {
@@ -1060,7 +1174,9 @@ static PolicyWs policy_ws(void *ws, long long tokens, long long sequences, bool 
     at += ids ? round_up256(tokens * 4) : 0;
     w.cnt.parts = reinterpret_cast<unsigned long long *>(p + at);
     w.cnt.n_parts = 0;
-    w.bytes = at + round_up256((long long)sm_count() * 2 * sizeof(unsigned long long));
+    w.cnt.places = reinterpret_cast<Place *>(p + at);  // with sequences there are no parts
+    const long long parts = (long long)sm_count() * 2 * sizeof(unsigned long long);
+    w.bytes = at + round_up256(parts > places_bytes() ? parts : places_bytes());
     return w;
 }
 
@@ -1092,6 +1208,23 @@ static CountArgs count_args(const PolicyWs &w, const uint8_t *mask, Idx labels, 
                             long long sequences, const PolicyRule &rule) {
     return CountArgs{mask,   labels, tokens, off, sequences, rule.by_sequence != 0, on4(mask),
                      w.cnt,  rule.by_sequence ? w.zero_bytes : 32};
+}
+// The kernels that count, for a kernel to follow.
+static int launch_counts(CountArgs &n, cudaStream_t st) {
+    if (!n.off.p) {
+        n.cnt.n_parts = grid_of(n.T, KEPT_THREADS * 4, sm_count() * 2);
+        n.cut = cut_of(n.T, (long long)n.cnt.n_parts * (KEPT_THREADS / 32));
+        WGB_PDL("k_policy_kept", k_policy_kept, dim3(n.cnt.n_parts), dim3(KEPT_THREADS), 0, st, n);
+    } else if (n.T + (n.by_sequence ? n.S : 0) <= ONE_BLOCK) {
+        n.cut = cut_of(n.T, BLOCK_THREADS / 32);
+        WGB_PDL("k_policy_count_block", k_policy_count_block, dim3(1), dim3(BLOCK_THREADS), 0, st, n);
+    } else {
+        WGB_PDL("k_policy_zero", k_policy_zero, dim3(part_grid(n.zero_bytes / 16, 1024)), dim3(GRID_THREADS), 0, st, n);
+        const int grid = walk_grid(n.T);
+        n.cut = cut_of(n.T, grid * (GRID_THREADS / 32));
+        WGB_PDL("k_policy_count", k_policy_count, dim3(grid), dim3(GRID_THREADS), 0, st, n);
+    }
+    return WGB_OK;
 }
 }  // namespace wgb
 
@@ -1129,7 +1262,15 @@ extern "C" int wgb_policy_loss(const float *logp, const float *old_logp, const f
     a.stats = stats;
     a.partial = w.partial;
     a.whole = on16(logp) && on16(old_logp) && (adv_by_sequence || on16(advantages)) && on16(ref_logp) && on16(grad_logp);
-    static int cache[64];
-    return launch_all("k_policy_tokens", k_policy_tokens<true, GRID_THREADS>, k_policy_tokens<false, BLOCK_THREADS>,
-                      tokens + (by_sequence ? sequences : 0), cache, a, as_stream(stream));
+    cudaStream_t st = as_stream(stream);
+    if (tokens + (by_sequence ? sequences : 0) <= ONE_BLOCK) {
+        a.count.cut = cut_of(tokens, BLOCK_THREADS / 32);
+        WGB_PDL("k_policy_tokens_block", k_policy_tokens_block, dim3(1), dim3(BLOCK_THREADS), 0, st, a);
+        return WGB_OK;
+    }
+    WGB_TRY(launch_counts(a.count, st));
+    const int grid = walk_grid(tokens);
+    a.count.cut = cut_of(tokens, grid * (GRID_THREADS / 32));
+    WGB_PDL("k_policy_tokens", k_policy_tokens, dim3(grid), dim3(GRID_THREADS), 0, st, a);
+    return WGB_OK;
 }
