@@ -503,11 +503,15 @@ __device__ __forceinline__ uint4 word_grad(const uint4 &w, const RowGrad &r, int
     }
     return Vec<T>::pack(o);
 }
-// One element, the same.
+// One element, the same, without the label's g.
+template <bool GE>
+__device__ __forceinline__ float one_grad(float x, const RowGrad &r) {
+    const float d = fmaf(x - r.top, r.c, -r.b), p = exp2_fast(d);
+    return -p * (GE ? fmaf(fmaxf(d, D_FLOOR), r.ge * LN2F, fmaf(r.ge, r.ent, r.g)) : r.g);
+}
 template <bool GE>
 __device__ __forceinline__ float one_grad(float x, const RowGrad &r, bool label) {
-    const float d = fmaf(x - r.top, r.c, -r.b), p = exp2_fast(d);
-    const float v = -p * (GE ? fmaf(fmaxf(d, D_FLOOR), r.ge * LN2F, fmaf(r.ge, r.ent, r.g)) : r.g);
+    const float v = one_grad<GE>(x, r);
     return r.zero ? 0.0f : label ? v + r.g : v;
 }
 // A row's gradient element by element, by threads tid, tid + n ...
@@ -605,9 +609,9 @@ __device__ __forceinline__ bool row_resum(const RowIn &r) { return r.kept && fab
 
 // From a row's sums (ROW_GRAD: from its lse, or from sums if `summed`) to what
 // it writes and to its gradient.  `scaled`: sum.m is in the units of d.
-template <int OP, bool ENT>
+template <int OP, bool ENT, typename ACC>
 __device__ __forceinline__ RowGrad row_close(const RowsArgs &a, const RowIn &in, const RowSum &sum, bool summed, bool scaled,
-                                             float x_y, long long i, bool leader, float inv_t, float c, double *tot) {
+                                             float x_y, long long i, bool leader, float inv_t, float c, ACC *tot) {
     RowGrad r{0.0f, c, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, !in.kept, !scaled};
     if (OP == ROW_GRAD) {
         r.zero = r.zero || in.a0 == -INFINITY;
@@ -624,7 +628,7 @@ __device__ __forceinline__ RowGrad row_close(const RowsArgs &a, const RowIn &in,
     const float l2 = none ? 0.0f : log2f(sum.s);
     const float d_y = scaled ? fmaf(x_y, c, -sum.m) : (x_y - sum.m) * c;
     const float lp = !in.kept ? 0.0f : none ? -INFINITY : (d_y - l2) * LN2F;
-    const float h = !in.kept || none ? 0.0f : ENT ? (l2 - sum.t / sum.s) * LN2F : 0.0f;
+    const float h = !in.kept || none ? 0.0f : ENT ? (l2 - __fdividef(sum.t, sum.s)) * LN2F : 0.0f;
     if (leader) {
         a.logp[i] = lp;
         if (OP == ROW_LOGP) {
@@ -643,10 +647,10 @@ __device__ __forceinline__ RowGrad row_close(const RowsArgs &a, const RowIn &in,
         r.b2 = sum.m + l2;
         r.zero = none;
         if (leader) {
-            tot[0] += (double)w * p.pg;
-            tot[1] += (double)w * p.kl;
-            tot[2] += (double)w * h;
-            tot[3] += (double)w * p.cut;
+            tot[0] += (ACC)w * (ACC)p.pg;
+            tot[1] += (ACC)w * (ACC)p.kl;
+            tot[2] += (ACC)w * (ACC)h;
+            tot[3] += (ACC)w * (ACC)p.cut;
         }
     }
     return r;
@@ -1203,11 +1207,14 @@ __global__ void __launch_bounds__(TILE_ROWS) k_rows_tile(const __grid_constant__
     const float inv_t = 1.0f / a.temperature, c = (float)LOG2E * inv_t;
     LateWeight<OP> weight;
     double tot[POL_STATS] = {};
+    float some[POL_STATS] = {};  // of up to 16 rows
+    int rows_in = 0;
     const bool dense = a.stride == K, dense_out = a.grad_stride == K;
     const bool whole = reinterpret_cast<uintptr_t>(logits) % 16 == 0, whole_out = reinterpret_cast<uintptr_t>(grad) % 16 == 0;
     const int words = K * (int)sizeof(T) / 4, g = words & -words;
     const int turn = K * (int)sizeof(T) % 4 || g == 1 ? 0 : tid / (32 / (g < 32 ? g : 32)) * (4 / (int)sizeof(T)) % K;
     T *mine = tile + tid * K;
+    T *const head = mine + turn, *const wrapped = head - K;  // element j: head[j], from K - turn on wrapped[j]
     for (long long i0 = (long long)blockIdx.x * TILE_ROWS; i0 < a.rows; i0 += (long long)gridDim.x * TILE_ROWS) {
         const int n = (int)(a.rows - i0 < TILE_ROWS ? a.rows - i0 : TILE_ROWS);
         const long long i = i0 + tid;
@@ -1216,51 +1223,71 @@ __global__ void __launch_bounds__(TILE_ROWS) k_rows_tile(const __grid_constant__
         if (dense) {
             tile_in(tile, logits + i0 * K, n * K, whole);
             __syncthreads();
+        } else if (live) {
+            for (int j = 0; j < K; ++j) mine[j] = logits[i * a.stride + j];
         }
         RowIn in = row_open<OP>(a, raw);
         float x[KM];
-        if (live) {
-            const T *from = dense ? mine : logits + i * a.stride;
-            int at = turn;
+        RowSum sum = row_none();
 #pragma unroll
-            for (int j = 0; j < KM; ++j) {
-                x[j] = j < K ? Vec<T>::to(from[at]) : -INFINITY;
-                at = at + 1 < K ? at + 1 : 0;
+        for (int q = 0; q < KM; q += 4) {
+#pragma unroll
+            for (int j = q; j < q + 4; ++j) x[j] = -INFINITY;
+            if (q < K) {  // by fours: what is past K then costs little
+#pragma unroll
+                for (int j = q; j < q + 4; ++j) {
+                    if (j < K && live) x[j] = Vec<T>::to((j < K - turn ? head : wrapped)[j]);
+                    sum.m = fmaxf(sum.m, x[j]);
+                }
             }
         }
-        RowSum sum = row_none();
         const bool summed = OP == ROW_GRAD ? row_resum(in) : in.kept;
-        if (summed) {
-#pragma unroll
-            for (int j = 0; j < KM; ++j) sum.m = fmaxf(sum.m, x[j]);
+        if (OP != ROW_GRAD || __any_sync(0xffffffffu, summed)) {
             const float top = finite_top(sum.m);
 #pragma unroll
-            for (int j = 0; j < KM; ++j) {
-                const float d = (x[j] - top) * c, e = exp2_fast(d);
-                sum.s += e;
-                if (ENT && OP != ROW_GRAD) sum.t = fmaf(e, fmaxf(d, D_FLOOR), sum.t);
+            for (int q = 0; q < KM; q += 4)
+                if (q < K) {
+#pragma unroll
+                    for (int j = q; j < q + 4; ++j) {
+                        const float d = (x[j] - top) * c, e = exp2_fast(d);
+                        sum.s += e;
+                        if (ENT && OP != ROW_GRAD) sum.t = fmaf(e, fmaxf(d, D_FLOOR), sum.t);
+                    }
+                }
+        }
+        const float x_y = !in.kept || in.y >= K ? NAN : Vec<T>::to(mine[in.y]);
+        weight.set(a, in);
+        const RowGrad r = row_close<OP, ENT>(a, in, sum, summed, false, x_y, i, live, inv_t, c, some);
+        if (OP == ROW_POLICY && ++rows_in == 16) {
+            rows_in = 0;
+            for (int k = 0; k < POL_STATS; ++k) {
+                tot[k] += (double)some[k];
+                some[k] = 0.0f;
             }
         }
-        const float x_y = OP == ROW_GRAD || !in.kept || in.y >= K ? NAN : Vec<T>::to(dense ? mine[in.y] : logits[i * a.stride + in.y]);
-        weight.set(a, in);
-        const RowGrad r = row_close<OP, ENT>(a, in, sum, summed, false, x_y, i, live, inv_t, c, tot);
         if (OP != ROW_LOGP) {
             if (live) {
-                T *to = dense_out ? mine : grad + i * a.grad_stride;
-                int at = turn;
 #pragma unroll
-                for (int j = 0; j < KM; ++j) {
-                    if (j < K) to[at] = Vec<T>::from(one_grad<ENT>(x[j], r, at == in.y));
-                    at = at + 1 < K ? at + 1 : 0;
-                }
+                for (int q = 0; q < KM; q += 4)
+                    if (q < K) {
+#pragma unroll
+                        for (int j = q; j < q + 4; ++j) {
+                            const float v = r.zero ? 0.0f : one_grad<ENT>(x[j], r);
+                            if (j < K) (j < K - turn ? head : wrapped)[j] = Vec<T>::from(v);
+                        }
+                    }
+                if (!r.zero && in.y < K) mine[in.y] = Vec<T>::from(one_grad<ENT>(x_y, r) + r.g);
             }
             if (dense_out) {
                 __syncthreads();
                 tile_out(tile, grad + i0 * K, n * K, whole_out);
+            } else if (live) {
+                for (int j = 0; j < K; ++j) grad[i * a.grad_stride + j] = mine[j];
             }
         }
         __syncthreads();
     }
+    for (int k = 0; k < POL_STATS; ++k) tot[k] += (double)some[k];
     if (OP == ROW_POLICY) policy_end_block(tot, a.rule, a.cnt.ticket, a.partial, a.stats, dscratch);
 }
 

@@ -108,29 +108,32 @@ struct Sums {
 };
 // The same memory for terms of at most `bound` in magnitude, n of them at most:
 // one addition to one of two 64-bit numbers, each a multiple of a power of two.
-// Terms from 2^-17 bound on count in units of bound 2^-62 n (2^-25 of the term or
-// less), smaller ones in units 2^17 times finer.
+// Terms from 2^-17 bound on count in units of bound 2^-62 n (n up to 2^21: 2^-25
+// of the term or less), smaller ones in units 2^17 times finer.
 struct GridSums {
     Sums s;
-    double unit, inv, small;  // 1 / unit of the first number, the unit; below `small`: the second
+    float unit, fine_unit, small;  // 1 / units of the two numbers; below `small`: the second
+    double inv;                    // the first unit
     __device__ __forceinline__ GridSums(const Sums &of, float bound, long long n) : s(of) {
-        int e = 0, m = 0;
+        int e = 0;
         bound = fminf(bound, 3.4028234e38f);
-        frexpf(bound, &e);             // bound <= 2^e
-        frexp((double)n, &m);          // n < 2^m
-        const int k = 62 - m - e;
-        unit = ldexp(1.0, k);
+        frexpf(bound, &e);                         // bound <= 2^e
+        if (e < -24) e = -24;                      // the units below stay within fp32's range
+        const int k = 62 - (64 - __clzll(n)) - e;  // n < 2^(64 - clz)
+        unit = ldexpf(1.0f, k);
+        fine_unit = ldexpf(1.0f, k + 17);
         inv = ldexp(1.0, -k);
-        small = ldexp((double)bound, -17);
+        small = ldexpf(1.0f, e - 17);
     }
+    // A power of two times v is exact; the conversion is the one rounding.
     __device__ __forceinline__ void add(long long i, float v) const {
-        const double u = fabs((double)v);
-        if (!(u < 1e300)) {
+        const float u = fabsf(v);
+        if (!(u < INFINITY)) {
             atomicOr(s.odd + (i >> 2), (u != u ? 4u : v > 0 ? 1u : 2u) << (8 * (i & 3)));
             return;
         }
         const bool fine = u < small;
-        const long long n = __double2ll_rn((double)v * (fine ? unit * 131072.0 : unit));
+        const long long n = __float2ll_rn(v * (fine ? fine_unit : unit));
         if (n) atomicAdd(s.lo_hi + 2 * i + fine, (unsigned long long)n);
     }
     __device__ __forceinline__ double value(long long i) const {
@@ -375,6 +378,13 @@ __device__ __forceinline__ void range_by_seq(const Idx &off, long long S, const 
 }
 
 // --------------------------------------------------------- preference --
+// e^x as 2^(x log2 e): relative error 2^-22 and 2^-24 |x|.
+__device__ __forceinline__ float exp_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504088896340736f));
+    return r;
+}
+
 struct PairRule {
     int kind;  // 0 sigmoid, 1 hinge, 2 square
     float beta, smoothing;
@@ -388,9 +398,10 @@ __device__ __forceinline__ PairTerm pair_term(const PairRule &r, float x) {
     const float h = r.beta * x;
     if (r.kind == 0) {
         // -log sigmoid(h) = softplus(-h); sigmoid(-h) = e^-|h| or 1 over 1 + e^-|h|
-        const float e = expf(-fabsf(h));
-        const float sp = log1pf(e);
-        const float inv = 1.0f / (1.0f + e);
+        const float e = exp_fast(-fabsf(h));
+        // log(1 + e): a series where 1 + e would lose e's digits (e^4 / 5 is left out)
+        const float sp = e < 0.03f ? e * fmaf(e, fmaf(e, fmaf(e, -0.25f, 1.0f / 3), -0.5f), 1.0f) : __logf(1.0f + e);
+        const float inv = __fdividef(1.0f, 1.0f + e);
         const float up = h >= 0 ? e * inv : inv;    // sigmoid(-h)
         const float down = h >= 0 ? inv : e * inv;  // sigmoid(h)
         p.loss = sp + (h >= 0 ? r.smoothing * h : (r.smoothing - 1.0f) * h);
@@ -433,12 +444,18 @@ struct PrefArgs {
     Cut cut;
 };
 
-// Score of sequence q: its sum (or mean) of log ratios; NaN out of range.
-__device__ __forceinline__ double seq_score(const PrefArgs &a, long long q) {
+// Score of sequence q: its sum (or mean) of log ratios, or (not RAGGED) row q's
+// difference; NaN out of range.
+template <bool RAGGED> using Score = std::conditional_t<RAGGED, double, float>;
+template <bool RAGGED>
+__device__ __forceinline__ Score<RAGGED> seq_score(const PrefArgs &a, long long q) {
     if (q < 0 || q >= a.S) return NAN;
-    if (!a.off.p) return (double)(a.ref ? a.diff : a.logp)[q];
-    const double v = a.scores.value(q);
-    return a.rule.average && a.count[q] ? v / (double)a.count[q] : v;
+    if constexpr (RAGGED) {
+        const double v = a.scores.value(q);
+        return a.rule.average && a.count[q] ? v / (double)a.count[q] : v;
+    } else {
+        return (a.ref ? a.diff : a.logp)[q];
+    }
 }
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -506,15 +523,16 @@ __device__ __forceinline__ void pref_sums(const PrefArgs &a) {
         });
 }
 // Losses of the pairs, and their gradients to the sequences.
-template <int NT>
+template <bool RAGGED, int NT>
 __device__ __forceinline__ void pref_pairs(const PrefArgs &a, double *scratch) {
+    using S = Score<RAGGED>;
     const long long me = (long long)blockIdx.x * NT + threadIdx.x, all = (long long)gridDim.x * NT;
     const bool bounded = a.rule.kind != 2;
     const GridSums grid_sums = pref_grid_sums(a);
     double total = 0.0;
     for (long long p0 = me; p0 < a.P; p0 += all * PAIR_EACH) {
         long long c[PAIR_EACH], r[PAIR_EACH];
-        double dc[PAIR_EACH], dr[PAIR_EACH];
+        S dc[PAIR_EACH], dr[PAIR_EACH];
         float wt[PAIR_EACH];
 #pragma unroll
         for (int e = 0; e < PAIR_EACH; ++e) {
@@ -525,28 +543,29 @@ __device__ __forceinline__ void pref_pairs(const PrefArgs &a, double *scratch) {
         }
 #pragma unroll
         for (int e = 0; e < PAIR_EACH; ++e) {
-            dc[e] = seq_score(a, c[e]);
-            dr[e] = seq_score(a, r[e]);
+            dc[e] = seq_score<RAGGED>(a, c[e]);
+            dr[e] = seq_score<RAGGED>(a, r[e]);
         }
+        float some = 0.0f;  // of PAIR_EACH pairs
 #pragma unroll
         for (int e = 0; e < PAIR_EACH; ++e) {
             const long long p = p0 + e * all;
             if (p >= a.P) break;
             const PairTerm t = pair_term(a.rule, (float)(dc[e] - dr[e]));
-            total += (double)wt[e] * (double)t.loss;
-            a.chosen_reward[p] = (float)(a.rule.beta * dc[e]);
-            a.rejected_reward[p] = (float)(a.rule.beta * dr[e]);
+            some = fmaf(wt[e], t.loss, some);
+            a.chosen_reward[p] = (float)((S)a.rule.beta * dc[e]);
+            a.rejected_reward[p] = (float)((S)a.rule.beta * dr[e]);
             const bool in_c = c[e] >= 0 && c[e] < a.S, in_r = r[e] >= 0 && r[e] < a.S;
+            const float g = wt[e] * t.slope;
             if (bounded) {
-                const float g = wt[e] * t.slope;
                 if (in_c) grid_sums.add(c[e], g);
                 if (in_r) grid_sums.add(r[e], -g);
             } else {
-                const double g = (double)wt[e] * (double)t.slope;
-                if (in_c) a.grads.add(c[e], g);
-                if (in_r) a.grads.add(r[e], -g);
+                if (in_c) a.grads.add(c[e], (double)g);
+                if (in_r) a.grads.add(r[e], -(double)g);
             }
         }
+        total += (double)some;
     }
     total = block_sum(total, scratch);
     if (threadIdx.x == 0) a.partial[blockIdx.x] = total;
@@ -619,7 +638,8 @@ __global__ void __launch_bounds__(GRID_THREADS) k_pref_part(const __grid_constan
     part_begin();
     if (PART == 0) pref_start<GRID_THREADS>(a);
     if (PART == 1) pref_sums(a);
-    if (PART == 2) pref_pairs<GRID_THREADS>(a, scratch);
+    if (PART == 2) pref_pairs<true, GRID_THREADS>(a, scratch);
+    if (PART == 4) pref_pairs<false, GRID_THREADS>(a, scratch);
     if (PART == 3) pref_grad<GRID_THREADS>(a, scratch);
 }
 __global__ void __launch_bounds__(BLOCK_THREADS) k_pref_block(const __grid_constant__ PrefArgs a) {
@@ -631,19 +651,13 @@ __global__ void __launch_bounds__(BLOCK_THREADS) k_pref_block(const __grid_const
         pref_sums(a);
         __syncthreads();
     }
-    pref_pairs<BLOCK_THREADS>(a, scratch);
+    if (a.off.p) pref_pairs<true, BLOCK_THREADS>(a, scratch);
+    else pref_pairs<false, BLOCK_THREADS>(a, scratch);
     __syncthreads();
     pref_grad<BLOCK_THREADS>(a, scratch);
 }
 
 // ------------------------------------------------------------- policy --
-// e^x as 2^(x log2 e): relative error 2^-22 and 2^-24 |x|.
-__device__ __forceinline__ float exp_fast(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504088896340736f));
-    return r;
-}
-
 struct PolicyRule {
     float clip_hi, clip_lo, log_hi, log_lo;  // 1 + high, 1 - low and their logarithms
     float kl_coef, ent_coef, grad_scale;
@@ -1148,7 +1162,8 @@ extern "C" int wgb_preference_loss(const float *logp, const float *ref_logp, int
     a.n_partial = part_grid(pairs, GRID_THREADS);
     WGB_PDL("k_pref_part", k_pref_part<0>, dim3(start), nt, 0, st, a);
     if (offsets) WGB_PDL("k_pref_part", k_pref_part<1>, dim3(tok), nt, 0, st, a);
-    WGB_PDL("k_pref_part", k_pref_part<2>, dim3(a.n_partial), nt, 0, st, a);
+    if (offsets) WGB_PDL("k_pref_part", k_pref_part<2>, dim3(a.n_partial), nt, 0, st, a);
+    else WGB_PDL("k_pref_part", k_pref_part<4>, dim3(a.n_partial), nt, 0, st, a);
     WGB_PDL("k_pref_part", k_pref_part<3>, dim3(tok), nt, 0, st, a);
     return WGB_OK;
 }
