@@ -473,11 +473,13 @@ __device__ __noinline__ RowSum careful_sum(const T *row, long long K, int tid, f
 // the gradient's own rounding.
 struct RowGrad {
     float top, c, b, b2, g, ge, ent;
+    float x_y;     // the label's logit
     bool zero;     // left out, or nothing but -inf
     bool careful;  // not plain
 };
+// Without the label's g, which whoever writes the label's word adds after.
 template <typename T, bool GE>
-__device__ __forceinline__ uint4 word_grad(const uint4 &w, const RowGrad &r, int y /* element of the label, or -1 */) {
+__device__ __forceinline__ uint4 word_grad(const uint4 &w, const RowGrad &r) {
     constexpr int N = Vec<T>::N;
     F2 f[N / 2];
     float o[N];
@@ -495,11 +497,6 @@ __device__ __forceinline__ uint4 word_grad(const uint4 &w, const RowGrad &r, int
         const float2 v = f2_split(f2_mul(p, h));
         o[2 * k] = v.x;
         o[2 * k + 1] = v.y;
-    }
-    if (y >= 0) {
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (k == y) o[k] += r.g;
     }
     return Vec<T>::pack(o);
 }
@@ -523,8 +520,8 @@ template <typename T, bool GE, typename J>
 __device__ __forceinline__ void word_emit(const RowWords<T, J> &rw, T *out, J q, const uint4 &w, const RowGrad &r,
                                           int y) {
     const J k = (J)y - (q * Vec<T>::N - rw.s);
-    rw.store(out, q, r.zero ? make_uint4(0u, 0u, 0u, 0u)
-                            : word_grad<T, GE>(w, r, k >= 0 && k < Vec<T>::N && y < rw.K ? (int)k : -1));
+    rw.store(out, q, r.zero ? make_uint4(0u, 0u, 0u, 0u) : word_grad<T, GE>(w, r));
+    if (k >= 0 && k < Vec<T>::N && y < rw.K && !r.zero) out[y] = Vec<T>::from(one_grad<GE>(r.x_y, r, true));
 }
 
 // --------------------------------------------------------- rows, by call --
@@ -612,7 +609,7 @@ __device__ __forceinline__ bool row_resum(const RowIn &r) { return r.kept && fab
 template <int OP, bool ENT, typename ACC>
 __device__ __forceinline__ RowGrad row_close(const RowsArgs &a, const RowIn &in, const RowSum &sum, bool summed, bool scaled,
                                              float x_y, long long i, bool leader, float inv_t, float c, ACC *tot) {
-    RowGrad r{0.0f, c, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, !in.kept, !scaled};
+    RowGrad r{0.0f, c, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, x_y, !in.kept, !scaled};
     if (OP == ROW_GRAD) {
         r.zero = r.zero || in.a0 == -INFINITY;
         r.g = in.y < a.K ? in.a1 * inv_t : NAN;
@@ -731,7 +728,7 @@ __global__ void __launch_bounds__(NT, GL > 32 ? 1024 / NT : 4) k_rows(const __gr
         const RowWords<T, int> rw(row, OP == ROW_LOGP ? row : out, (int)a.K);
         const int words = rw.words();
         const int per = (words + GL - 1) / GL;  // words of a thread, at most U
-        const float x_y = OP == ROW_GRAD ? 0.0f : label_logit(row, in, a.K);
+        const float x_y = label_logit(row, in, a.K);
         uint4 w[U];
         rw.load(w, tid, GL, in.kept ? per : 0, words);
         next = row_fetch<OP>(a, i + step);
@@ -801,7 +798,7 @@ __global__ void __launch_bounds__(NT, 2) k_rows_long(const __grid_constant__ Row
         T *out = OP == ROW_LOGP ? nullptr : grad + i * a.grad_stride;
         const RowWords<T, long long> rw(row, OP == ROW_LOGP ? row : out, a.K);
         const long long words = rw.words();
-        const float x_y = OP == ROW_GRAD ? 0.0f : label_logit(row, in, a.K);
+        const float x_y = label_logit(row, in, a.K);
         const bool summed = OP == ROW_GRAD ? row_resum(in) : in.kept;
         RowSum sum = row_none();
         bool scaled = false, careful = OP == ROW_GRAD && summed;
@@ -996,7 +993,7 @@ __global__ void __launch_bounds__(RING_NT, ring_blocks<OP>()) k_rows_ring(const 
             const T *row = logits + i * a.stride;
             T *out = OP == ROW_LOGP ? nullptr : grad + i * a.grad_stride;
             const RowRec rec = row_rec<T, CL>(row, K, i, in.y, rank);
-            float x_y = 0.0f;
+            float x_y = OP == ROW_GRAD ? label_logit(row, in, a.K) : 0.0f;
             RowSum sum = row_none();
             bool scaled = false;
             const bool resum = OP == ROW_GRAD && row_resum(in);
@@ -1141,20 +1138,25 @@ __global__ void __launch_bounds__(RING_NT, ring_blocks<OP>()) k_rows_ring(const 
                 }
                 continue;
             }
-            // this thread's first word, and the label's word from there
             uint4 *o = reinterpret_cast<uint4 *>(out + rec.head) + rec.begin + threadIdx.x;
-            const int yq = y >= rec.head ? (y - rec.head) / N - rec.begin - (int)threadIdx.x : -1, yk = (y - rec.head) % N;
-            for (int at = 0; at < rec.n; at += SW) {
+            for (int at = 0; at < rec.n; at += SW, o += SW) {
                 read(w, slot, parity, rec.n - at);
                 release();
                 raise_floor(w);
+                if (!r.zero && rec.n - at >= SW) {
 #pragma unroll
-                for (int u = 0; u < LW; ++u) {
-                    const int q = at + u * RING_CONS;
-                    if (q + (int)threadIdx.x < rec.n)
-                        o[q] = r.zero ? make_uint4(0u, 0u, 0u, 0u) : word_grad<T, ENT>(w[u], r, q == yq ? yk : -1);
+                    for (int u = 0; u < LW; ++u) o[u * RING_CONS] = word_grad<T, ENT>(w[u], r);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < LW; ++u)
+                        if (at + u * RING_CONS + (int)threadIdx.x < rec.n)
+                            o[u * RING_CONS] = r.zero ? make_uint4(0u, 0u, 0u, 0u) : word_grad<T, ENT>(w[u], r);
                 }
             }
+            // the label, by the thread that wrote its word
+            const int yq = y >= rec.head ? (y - rec.head) / N - rec.begin : -1;
+            if (!r.zero && yq >= 0 && yq < rec.n && yq % RING_CONS == (int)threadIdx.x)
+                out[y] = Vec<T>::from(one_grad<ENT>(r.x_y, r, true));
         }
     }
     if (lost)  // copies that did not arrive in time may still do so
