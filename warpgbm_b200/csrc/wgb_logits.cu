@@ -773,9 +773,9 @@ __global__ void __launch_bounds__(NT, GL > 32 ? 1024 / NT : 4) k_rows(const __gr
     }
 }
 
-// Rows that neither of the others takes (longer than a cluster's registers, or
-// a gradient aligned otherwise than its row): a block reads its row, and for
-// the gradient reads it again, from L2 as a rule.
+// Rows that neither of the others takes (a gradient aligned otherwise than its
+// row, or 2^30 classes and more): a block reads its row, and for the gradient
+// reads it again, from L2 as a rule.
 template <typename T, int OP, bool ENT, int NT>
 __global__ void __launch_bounds__(NT, 2) k_rows_long(const __grid_constant__ RowsArgs a) {
     constexpr int U = 4;
@@ -852,15 +852,18 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, unsigned b
                  : "memory");
 }
 
-constexpr int RING_WARPS = 8;                 // that take words
-constexpr int RING_CONS = RING_WARPS * 32;
-constexpr int RING_NT = RING_CONS + 64;       // and one that copies and one that closes rows
-template <int OP> __host__ __device__ constexpr int ring_blocks() { return OP == ROW_LOGP ? 3 : 2; }  // of an SM
-template <int OP> __host__ __device__ constexpr int ring_lane_words() { return 4; }  // of a lane in a stage
-template <int OP> __host__ __device__ constexpr int ring_stages() { return OP == ROW_LOGP ? 4 : 6; }  // 192 KB of an SM
-template <int OP> __host__ __device__ constexpr int stage_words() { return RING_CONS * ring_lane_words<OP>(); }
-template <int OP> __host__ __device__ constexpr int ring_smem() { return ring_stages<OP>() * stage_words<OP>() * 16; }
-constexpr int RING_RECS = 8;                  // at least the stages
+// A ring for W warps that take words (8, or 16 in the one block of an SM), one
+// that copies and one that closes rows.
+template <int OP, int W>
+struct Ring {
+    static constexpr int CONS = W * 32, NT = CONS + 64;
+    static constexpr int BLOCKS = W == 16 ? 1 : OP == ROW_GRAD ? 2 : 3;   // of an SM
+    static constexpr int LANE_WORDS = 4;                                  // of a lane in a stage
+    static constexpr int STAGE = CONS * LANE_WORDS;                       // words
+    static constexpr int STAGES = W == 16 || OP == ROW_GRAD ? 6 : 4;      // 192 KB of an SM under way
+    static constexpr int SMEM = STAGES * STAGE * 16;
+};
+constexpr int RING_RECS = 8;  // at least the stages
 
 // A row on its way: which one, its aligned words, and this block's share of them.
 struct RowRec {
@@ -885,12 +888,16 @@ __device__ __forceinline__ RowRec row_rec(const T *row, int K, long long i, int 
 
 // Rows streamed through shared memory by a block, or by the CL blocks of a
 // cluster, which share each row.  One warp keeps a ring of stages full with bulk
-// copies of this row and the rows to come, so that HBM stays busy while sums
-// are joined and gradients written.  RING_WARPS warps form the sums and write
-// the gradients.  One warp turns joined sums into what a row writes, a row's
-// scalars loaded a row ahead, so that the others carry no work that is the same
-// for all.  ROW_POLICY keeps a row's stages until its gradient is written, so
-// that a row is read from HBM once.
+// copies of this row and the rows to come, so that HBM stays busy while sums are
+// joined and gradients written.  W warps form the sums and write the gradients.
+// One warp turns joined sums into what a row writes, a row's scalars loaded a row
+// ahead, so that the others carry no work that is the same for all.
+//
+// ROW_POLICY takes a row's words twice, for the sums and for the gradient; the
+// second time they come from L2, if the rows under way fit there (ring_team).
+// Keeping them on the chip instead, in a cluster's shared memory, took 442 us for
+// 4096 x 131072 bf16 against 390: the blocks of a cluster wait for one another
+// twice a row.
 //
 // In place a gradient is written only after the whole row is read: the row's own
 // words, its ends and the label's logit all go into what a warp puts.
@@ -901,12 +908,12 @@ __device__ __forceinline__ RowRec row_rec(const T *row, int K, long long i, int 
 // k (ROW_POLICY); ROW_LOGP's warps wait until row k is closed, and ROW_GRAD's
 // closing warp until all have read row k's desc.  A wait that runs out makes NaN
 // of the rows from there on.
-template <typename T, int OP, bool ENT, int CL>
-__global__ void __launch_bounds__(RING_NT, ring_blocks<OP>()) k_rows_ring(const __grid_constant__ RowsArgs a) {
+template <typename T, int OP, bool ENT, int W, int CL>
+__global__ void __launch_bounds__(Ring<OP, W>::NT, Ring<OP, W>::BLOCKS) k_rows_ring(const __grid_constant__ RowsArgs a) {
+    using R = Ring<OP, W>;
     constexpr int N = Vec<T>::N;
-    constexpr int LW = ring_lane_words<OP>();
-    constexpr int SW = stage_words<OP>();
-    constexpr int S = ring_stages<OP>();
+    constexpr int LW = R::LANE_WORDS, SW = R::STAGE, S = R::STAGES;
+    constexpr int RING_WARPS = W, RING_CONS = R::CONS;
     constexpr bool HALF = Vec<T>::HALF;
     constexpr bool SENT = ENT && OP != ROW_GRAD;
     static_assert(S <= RING_RECS, "a record for every stage");
@@ -960,12 +967,17 @@ __global__ void __launch_bounds__(RING_NT, ring_blocks<OP>()) k_rows_ring(const 
             const T *row = logits + i * a.stride;
             const RowRec r = row_rec<T, CL>(row, K, i, y, rank);
             const T *src = row + r.head + (long long)r.begin * N;
-            for (int at = 0; at < r.n; at += SW) {
+            // ROW_POLICY: once for the sums and once, then from L2, for the gradient
+            for (int at = 0, pass = OP == ROW_POLICY ? 0 : 1; pass < 2; at += SW) {
+                if (at >= r.n) {
+                    at = 0;
+                    if (++pass == 2) break;
+                }
                 if (round) bar_wait(&empty[slot], (round - 1) & 1, lost);
                 if (lost) break;
                 if (lane == 0) {
                     const unsigned bytes = 16u * (r.n - at < SW ? r.n - at : SW);
-                    if (at == 0) recs[k % RING_RECS] = r;
+                    if (at == 0 && (OP != ROW_POLICY || pass == 0)) recs[k % RING_RECS] = r;
                     bar_expect(&full[slot], bytes);
                     bulk_load(ring_mem + slot * SW, src + (long long)at * N, bytes, &full[slot]);
                 }
@@ -1097,17 +1109,11 @@ __global__ void __launch_bounds__(RING_NT, ring_blocks<OP>()) k_rows_ring(const 
                     const int at = lane < rec.head ? lane : lane >= 16 && tail + lane - 16 < K ? tail + lane - 16 : -1;
                     if (at >= 0) sh.add_one(Vec<T>::to(row[at]), c);
                 }
-                int s = slot;
-                unsigned ph = parity;
                 for (int at = 0; at < rec.n; at += SW) {
-                    read(w, s, ph, rec.n - at);
-                    if (OP == ROW_LOGP) release();
+                    read(w, slot, parity, rec.n - at);
+                    release();
                     raise_floor(w);
                     sh.template add<LW>(w, c);
-                    if (++s == S) {
-                        s = 0;
-                        ph ^= 1u;
-                    }
                 }
                 RowSum sum = lanes_join<32, SENT>(sh.sum(), HALF ? 1.0f : c);
                 if (lost) sum.s = NAN;
@@ -1341,17 +1347,21 @@ static int go_rows(const RowsArgs &a, int &grid, cudaStream_t st) {
     return launch_rows(k_rows<T, OP, ENT, GL, NT, U>, (a.rows + RPC - 1) / RPC, NT, 1, 0, cache, a, grid, st);
 }
 
-template <typename T, int OP, bool ENT, int CL>
+template <typename T, int OP, bool ENT, int W, int CL>
 static int go_ring(const RowsArgs &a, int &grid, cudaStream_t st) {
     static int cache[64];
-    constexpr int smem = ring_smem<OP>();
-    auto kernel = k_rows_ring<T, OP, ENT, CL>;
+    using R = Ring<OP, W>;
+    auto kernel = k_rows_ring<T, OP, ENT, W, CL>;
     int dev = 0;
     WGB_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !cache[dev])
-        WGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    return launch_rows(kernel, a.rows, RING_NT, CL, smem, cache, a, grid, st);
+        WGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM));
+    return launch_rows(kernel, a.rows, R::NT, CL, R::SMEM, cache, a, grid, st);
 }
+// Bytes of a row from which on ROW_POLICY gives an SM one row at a time: the rows
+// under way, three to an SM, would no longer be in L2 when they are read again
+// (65536 bf16 classes: 205 against 239 us for 4096 rows; 50000: 197 against 164).
+constexpr long long ONE_ROW = 112 << 10;
 
 template <typename T, int OP, bool ENT, int KM>
 static int go_tile(const RowsArgs &a, int &grid, cudaStream_t st) {
@@ -1377,18 +1387,16 @@ static int run_rows(const RowsArgs &a, int &grid, cudaStream_t st) {
     const bool alike = OP == ROW_LOGP || ((reinterpret_cast<uintptr_t>(a.logits) - reinterpret_cast<uintptr_t>(a.grad)) % 16 == 0 &&
                                           (a.rows <= 1 || (a.stride - a.grad_stride) * (long long)sizeof(T) % 16 == 0));
     if (alike && a.K < (1ll << 30)) {
-        const long long inner = a.K / N;  // whole words, at most
+        if constexpr (OP == ROW_POLICY) {
+            if (a.rows > 3 * sm_count() && a.K * (long long)sizeof(T) >= ONE_ROW) return go_ring<T, OP, ENT, 16, 1>(a, grid, st);
+        }
         int cl = 1;
-        if (OP == ROW_POLICY)  // a third of the stages is left for the rows to come
-            while (cl < 8 && inner > (long long)cl * stage_words<OP>() * (ring_stages<OP>() * 2 / 3)) cl *= 2;
         // few rows: more blocks to a row, while the SMs are not all taken
         while (cl < 8 && a.rows * cl * 2 <= sm_count()) cl *= 2;
-        if (OP != ROW_POLICY || inner <= (long long)cl * stage_words<OP>() * ring_stages<OP>()) {
-            if (cl == 1) return go_ring<T, OP, ENT, 1>(a, grid, st);
-            if (cl == 2) return go_ring<T, OP, ENT, 2>(a, grid, st);
-            if (cl == 4) return go_ring<T, OP, ENT, 4>(a, grid, st);
-            return go_ring<T, OP, ENT, 8>(a, grid, st);
-        }
+        if (cl == 1) return go_ring<T, OP, ENT, 8, 1>(a, grid, st);
+        if (cl == 2) return go_ring<T, OP, ENT, 8, 2>(a, grid, st);
+        if (cl == 4) return go_ring<T, OP, ENT, 8, 4>(a, grid, st);
+        return go_ring<T, OP, ENT, 8, 8>(a, grid, st);
     }
     static int cache[64];
     return launch_rows(k_rows_long<T, OP, ENT, 512>, a.rows, 512, 1, 0, cache, a, grid, st);
