@@ -474,6 +474,7 @@ __device__ __noinline__ RowSum careful_sum(const T *row, long long K, int tid, f
 struct RowGrad {
     float top, c, b, b2, g, ge, ent;
     float x_y;     // the label's logit
+    int y;
     bool zero;     // left out, or nothing but -inf
     bool careful;  // not plain
 };
@@ -609,7 +610,7 @@ __device__ __forceinline__ bool row_resum(const RowIn &r) { return r.kept && fab
 template <int OP, bool ENT, typename ACC>
 __device__ __forceinline__ RowGrad row_close(const RowsArgs &a, const RowIn &in, const RowSum &sum, bool summed, bool scaled,
                                              float x_y, long long i, bool leader, float inv_t, float c, ACC *tot) {
-    RowGrad r{0.0f, c, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, x_y, !in.kept, !scaled};
+    RowGrad r{0.0f, c, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, x_y, in.y, !in.kept, !scaled};
     if (OP == ROW_GRAD) {
         r.zero = r.zero || in.a0 == -INFINITY;
         r.g = in.y < a.K ? in.a1 * inv_t : NAN;
@@ -694,82 +695,217 @@ __device__ __forceinline__ void row_mend(RowSum &sum, bool &scaled, const T *row
     }
 }
 
-// Rows held in registers: GL lanes, or the NT threads of a block, hold a row in
-// U words each; the maximum, the sums and the gradient come out of the
-// registers.
-template <typename T, int OP, bool ENT, int GL, int NT, int U>
-__global__ void __launch_bounds__(NT, GL > 32 ? 1024 / NT : 4) k_rows(const __grid_constant__ RowsArgs a) {
-    constexpr bool BLOCK = GL > 32;
-    constexpr int RPC = BLOCK ? 1 : NT / GL;
+// A row that its gradient is aligned like, as aligned words and single elements
+// at both ends.
+struct RowCut {
+    int head, words, inner;  // elements before the words, words, elements in them
+    __device__ __forceinline__ int end(int k) const { return k < head ? k : k + inner; }  // k-th of the single elements
+};
+template <typename T>
+__device__ __forceinline__ RowCut row_cut(const T *row, int K) {
+    constexpr int N = Vec<T>::N;
+    RowCut r;
+    r.head = (int)((0u - (unsigned)(reinterpret_cast<uintptr_t>(row) / sizeof(T))) % N);
+    if (r.head > K) r.head = K;
+    r.words = (K - r.head) / N;
+    r.inner = r.words * N;
+    return r;
+}
+
+// All of a row that is not plain, by one warp.  Returns its share of the totals
+// (in lane 0).
+template <typename T, int OP, bool ENT>
+__device__ __noinline__ float4 careful_row(const RowsArgs &a, long long i, float w_all) {
+    const int lane = threadIdx.x & 31;
+    const float inv_t = 1.0f / a.temperature, c = (float)LOG2E * inv_t;
+    RowIn in = row_open<OP>(a, row_fetch<OP>(a, i));
+    if (OP == ROW_POLICY && !a.rule.by_sequence) in.a3 = w_all;
+    const T *row = static_cast<const T *>(a.logits) + i * a.stride;
+    const float x_y = label_logit(row, in, a.K);
+    const RowSum sum = careful_sum<T, 32, 32, ENT && OP != ROW_GRAD>(row, a.K, lane, c, nullptr);
+    float some[POL_STATS] = {};
+    const RowGrad r = row_close<OP, ENT>(a, in, sum, true, false, x_y, i, lane == 0, inv_t, c, some);
+    __syncwarp();
+    if (OP != ROW_LOGP) careful_grad<T, ENT>(row, static_cast<T *>(a.grad) + i * a.grad_stride, a.K, in.y, lane, 32, r);
+    return make_float4(some[0], some[1], some[2], some[3]);
+}
+
+// Rows of some tens to some thousands of classes: GL lanes take a row, U words
+// each, and a warp B batches of 32 / GL rows, one after another.  What a row does
+// once (its scalars, its logarithm, the loss) is done by a lane of its own for
+// all rows of the warp together: repeated by all lanes of a row it took most of
+// the time of short rows.  ROW_POLICY keeps the words in shared memory (8 KB a
+// warp) until the gradient, so that a row is read once.
+constexpr int WARP_NT = 128;
+template <typename T, int GL, int U, int B>
+struct Batch {
+    static constexpr int G = 32 / GL, ROWS = G * B, WARPS = WARP_NT / 32;
+    static constexpr int ENDS = (2 * Vec<T>::N - 2 + GL - 1) / GL;  // elements outside the aligned words, to a lane
+    static constexpr int SMEM = WARPS * B * 32 * (U * 16 + ENDS * 4);
+};
+template <typename T, int OP, bool ENT, int GL, int U, int B>
+__global__ void __launch_bounds__(WARP_NT, U > 8 ? 4 : 6) k_rows(const __grid_constant__ RowsArgs a) {
+    using Bt = Batch<T, GL, U, B>;
+    constexpr int G = Bt::G, RB = Bt::ROWS, WARPS = Bt::WARPS, E = Bt::ENDS, N = Vec<T>::N;
     constexpr bool SENT = ENT && OP != ROW_GRAD;  // the sums have an entropy
-    __shared__ float4 part[2][BLOCK ? NT / 32 : 1], again[BLOCK ? NT / 32 : 1];
-    __shared__ double dscratch[33];
+    constexpr bool PRE = U <= 4;                  // a batch's words are loaded while the batch before is worked on
+    extern __shared__ __align__(16) uint4 batch_mem[];
+    __shared__ float4 all_sums[WARPS][OP == ROW_GRAD ? 1 : RB];
+    __shared__ RowGrad all_desc[WARPS][OP == ROW_LOGP ? 1 : RB];
+    __shared__ double dscratch[33], all_tot[WARPS][POL_STATS];
     early_wait<OP>(a);
-    __shared__ double shared_tot[POL_STATS];  // a block's one leader keeps its totals out of the registers
-    double own_tot[POL_STATS] = {};
-    double *tot = BLOCK ? shared_tot : own_tot;
-    if (BLOCK && threadIdx.x < POL_STATS) shared_tot[threadIdx.x] = 0.0;
-    if (BLOCK) __syncthreads();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = lane % GL, group = lane / GL;
+    if (OP == ROW_POLICY && lane < POL_STATS) all_tot[warp][lane] = 0.0;
+    float4 *sums = all_sums[warp];
+    RowGrad *desc = all_desc[warp];
+    uint4 *kept_words = batch_mem + warp * (B * 32 * U) + lane;                                             // [B][U][32]
+    float *kept_ends = reinterpret_cast<float *>(batch_mem + WARPS * B * 32 * U) + warp * (B * 32 * E) + lane;  // [B][E][32]
     const T *logits = static_cast<const T *>(a.logits);
     T *grad = static_cast<T *>(a.grad);
-    const int tid = BLOCK ? threadIdx.x : threadIdx.x % GL;
     const float inv_t = 1.0f / a.temperature, c = (float)LOG2E * inv_t;
+    const int K = (int)a.K;
     LateWeight<OP> weight;
-    const long long step = (long long)gridDim.x * RPC;
-    int turn = 0;
-    const long long mine = (long long)blockIdx.x * RPC + (BLOCK ? 0 : threadIdx.x / GL);
-    RowRaw next = row_fetch<OP>(a, mine);
-    for (long long base = (long long)blockIdx.x * RPC; base < a.rows; base += step) {
-        const long long i = base + (BLOCK ? 0 : threadIdx.x / GL);
-        const bool live = i < a.rows;
-        RowIn in = row_open<OP>(a, next);
-        const T *row = logits + (live ? i : 0) * a.stride;
-        T *out = OP == ROW_LOGP ? nullptr : grad + (live ? i : 0) * a.grad_stride;
-        const RowWords<T, int> rw(row, OP == ROW_LOGP ? row : out, (int)a.K);
-        const int words = rw.words();
-        const int per = (words + GL - 1) / GL;  // words of a thread, at most U
-        const float x_y = label_logit(row, in, a.K);
-        uint4 w[U];
-        rw.load(w, tid, GL, in.kept ? per : 0, words);
-        next = row_fetch<OP>(a, i + step);
-        if (ENT) {
+    float some[POL_STATS] = {};  // of up to 16 of this lane's rows
+    int rows_in = 0;
+    auto flush = [&]() {
+        rows_in = 0;
 #pragma unroll
-            for (int u = 0; u < U; ++u) w[u] = Vec<T>::floored(w[u]);
+        for (int k = 0; k < POL_STATS; ++k) {
+            const double v = warp_sum((double)some[k]);
+            if (lane == 0) all_tot[warp][k] += v;
+            some[k] = 0.0f;
         }
-        RowSum sum = row_none();
-        bool scaled = false, summed = true, careful = false;
-        if (OP == ROW_GRAD) {
-            careful = summed = row_resum(in);
-            if (BLOCK ? summed : __any_sync(0xffffffffu, summed)) {
-                sum = careful_sum<T, GL, NT, false>(row, summed ? a.K : 0, tid, c, part[turn]);
-                turn ^= 1;
+    };
+    const long long step = (long long)gridDim.x * WARPS * RB;
+    long long base = ((long long)blockIdx.x * WARPS + warp) * RB;
+    auto fetch = [&](long long first) { return row_fetch<OP>(a, lane < RB ? first + lane : a.rows); };
+    RowRaw raw = fetch(base);
+    struct Words {
+        uint4 w[U];
+        float ends[E];
+    };
+    for (; base < a.rows; base += step) {
+        // this lane's row
+        const long long mine = base + (lane < RB ? lane : 0);
+        const bool live = lane < RB && mine < a.rows;
+        RowIn in = row_open<OP>(a, raw);
+        const unsigned through = __ballot_sync(0xffffffffu, row_passes(raw));
+        auto load = [&](int b, Words &x) {
+            const int r = b * G + group;
+            const bool in_row = through >> r & 1u;
+            const T *row = logits + (in_row ? base + r : 0) * a.stride;
+            const RowCut cut = row_cut(row, K);
+            const uint4 *from = reinterpret_cast<const uint4 *>(row + cut.head) + tid;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                x.w[u] = make_uint4(Vec<T>::LOW, Vec<T>::LOW, Vec<T>::LOW, Vec<T>::LOW);
+                if (in_row && tid + u * GL < cut.words) x.w[u] = from[u * GL];
             }
-        } else if (!BLOCK || in.kept) {
-            Share<T, SENT> sh;
-            sh.template add<U>(w, c);
-            sum = group_join<GL, NT, SENT>(sh.sum(), Vec<T>::HALF ? 1.0f : c, part[turn]);
-            turn ^= 1;
-            row_mend<T, GL, NT, SENT>(sum, scaled, row, a.K, in.kept, tid, c, again);
-            careful = Vec<T>::HALF && in.kept && !scaled;
-        }
-        weight.set(a, in);
-        const RowGrad r = row_close<OP, ENT>(a, in, sum, summed, scaled, x_y, i, live && tid == 0, inv_t, c, tot);
-        if (!BLOCK) __syncwarp();  // in place: every lane has read its row before any writes
-        if (OP != ROW_LOGP && live) {
-            if (careful) {
-                careful_grad<T, ENT>(row, out, a.K, in.y, tid, GL, r);
-            } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int j = cut.end(tid + e * GL);
+                x.ends[e] = -INFINITY;
+                if (in_row && j < K) x.ends[e] = Vec<T>::to(row[j]);
+            }
+        };
+        Words x, ahead;
+        if (PRE) load(0, ahead);
+        const float x_y = label_logit(logits + (live ? mine : 0) * a.stride, in, a.K);
+        raw = fetch(base + step);
+        RowSum sum = row_none();
+        bool again = OP == ROW_GRAD && row_resum(in);
+        if (OP != ROW_GRAD) {
+#pragma unroll 1
+            for (int b = 0; b < B; ++b) {
+                if (PRE) {
+                    x = ahead;
+                    if (b + 1 < B) load(b + 1, ahead);
+                } else {
+                    load(b, x);
+                }
+                Share<T, SENT> sh;
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const int q = tid + u * GL;
-                    if (u < per && q < words) word_emit<T, ENT>(rw, out, q, w[u], r, in.y);
+                    if (ENT) x.w[u] = Vec<T>::floored(x.w[u]);
+                    if (OP == ROW_POLICY) kept_words[(b * U + u) * 32] = x.w[u];
                 }
+                sh.template add<U>(x.w, c);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    sh.add_one(x.ends[e], c);
+                    if (OP == ROW_POLICY) kept_ends[(b * E + e) * 32] = x.ends[e];
+                }
+                const RowSum s = lanes_join<GL, SENT>(sh.sum(), Vec<T>::HALF ? 1.0f : c);
+                if (tid == 0) sums[b * G + group] = make_float4(s.m, s.s, s.t, 0.0f);
+            }
+            __syncwarp();
+            const float4 v = sums[lane < RB ? lane : 0];
+            sum = RowSum{v.x, v.y, v.z};
+            again = Vec<T>::HALF && in.kept && !plain<T>(sum, c);
+        }
+        weight.set(a, in);
+        RowGrad r = row_close<OP, ENT>(a, in, sum, OP != ROW_GRAD, Vec<T>::HALF && OP != ROW_GRAD, x_y, mine, live && !again,
+                                       inv_t, c, some);
+        r.careful = again;
+        if (OP != ROW_LOGP && lane < RB) desc[lane] = r;
+        __syncwarp();
+        if (OP != ROW_LOGP) {
+#pragma unroll 1
+            for (int b = 0; b < B; ++b) {
+                const int k = b * G + group;
+                const long long i = base + k;
+                if (OP == ROW_POLICY) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) x.w[u] = kept_words[(b * U + u) * 32];
+#pragma unroll
+                    for (int e = 0; e < E; ++e) x.ends[e] = kept_ends[(b * E + e) * 32];
+                } else {
+                    if (PRE) {
+                        x = ahead;
+                        if (b + 1 < B) load(b + 1, ahead);
+                    } else {
+                        load(b, x);
+                    }
+                    if (ENT) {
+#pragma unroll
+                        for (int u = 0; u < U; ++u) x.w[u] = Vec<T>::floored(x.w[u]);
+                    }
+                }
+                const RowGrad q = desc[k];
+                if (i >= a.rows || q.careful) continue;
+                T *out = grad + i * a.grad_stride;
+                const RowCut cut = row_cut(out, K);  // aligned as the row is
+                uint4 *to = reinterpret_cast<uint4 *>(out + cut.head) + tid;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (tid + u * GL < cut.words) to[u * GL] = q.zero ? make_uint4(0u, 0u, 0u, 0u) : word_grad<T, ENT>(x.w[u], q);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const int j = cut.end(tid + e * GL);
+                    if (j < K) out[j] = Vec<T>::from(one_grad<ENT>(x.ends[e], q, j == q.y));
+                }
+                const int yq = q.y - cut.head;  // the label among the words: by the lane that wrote its word
+                if (!q.zero && yq >= 0 && yq < cut.inner && yq / N % GL == tid)
+                    out[q.y] = Vec<T>::from(one_grad<ENT>(q.x_y, q, true));
             }
         }
+        __syncwarp();
+        for (unsigned rest = __ballot_sync(0xffffffffu, again); rest; rest &= rest - 1) {
+            const float4 v = careful_row<T, OP, ENT>(a, base + __ffs(rest) - 1, weight.w);
+            if (lane == 0) {
+                some[0] += v.x;
+                some[1] += v.y;
+                some[2] += v.z;
+                some[3] += v.w;
+            }
+        }
+        if (OP == ROW_POLICY && ++rows_in == 16) flush();
     }
     if (OP == ROW_POLICY) {
-        if (!BLOCK) policy_end_block(own_tot, a.rule, a.cnt.ticket, a.partial, a.stats, dscratch);
-        else if (threadIdx.x < 32) policy_end(shared_tot, a.rule, a.cnt.ticket, a.partial, a.stats);
+        flush();
+        double tot[POL_STATS];
+        for (int k = 0; k < POL_STATS; ++k) tot[k] = lane == 0 ? all_tot[warp][k] : 0.0;
+        policy_end_block(tot, a.rule, a.cnt.ticket, a.partial, a.stats, dscratch);
     }
 }
 
@@ -777,7 +913,7 @@ __global__ void __launch_bounds__(NT, GL > 32 ? 1024 / NT : 4) k_rows(const __gr
 // row, or 2^30 classes and more): a block reads its row, and for the gradient
 // reads it again, from L2 as a rule.
 template <typename T, int OP, bool ENT, int NT>
-__global__ void __launch_bounds__(NT, 2) k_rows_long(const __grid_constant__ RowsArgs a) {
+__global__ void __launch_bounds__(NT, 1024 / NT) k_rows_long(const __grid_constant__ RowsArgs a) {
     constexpr int U = 4;
     constexpr bool SENT = ENT && OP != ROW_GRAD;
     __shared__ float4 part[2][NT / 32], again[NT / 32];
@@ -1340,11 +1476,13 @@ static int launch_rows(K kernel, long long units, int nt, int cl, int smem, int 
     return WGB_OK;
 }
 
-template <typename T, int OP, bool ENT, int GL, int NT, int U>
+template <typename T, int OP, bool ENT, int GL, int U, int B>
 static int go_rows(const RowsArgs &a, int &grid, cudaStream_t st) {
     static int cache[64];
-    constexpr int RPC = GL > 32 ? 1 : NT / GL;
-    return launch_rows(k_rows<T, OP, ENT, GL, NT, U>, (a.rows + RPC - 1) / RPC, NT, 1, 0, cache, a, grid, st);
+    using Bt = Batch<T, GL, U, B>;
+    constexpr int rows = Bt::WARPS * Bt::ROWS, smem = OP == ROW_POLICY ? Bt::SMEM : 0;
+    static_assert(smem <= 48 << 10, "no opt-in for more");
+    return launch_rows(k_rows<T, OP, ENT, GL, U, B>, (a.rows + rows - 1) / rows, WARP_NT, 1, smem, cache, a, grid, st);
 }
 
 template <typename T, int OP, bool ENT, int W, int CL>
@@ -1370,22 +1508,29 @@ static int go_tile(const RowsArgs &a, int &grid, cudaStream_t st) {
                        TILE_ROWS * KM * (int)sizeof(T), cache, a, grid, st);
 }
 
-// Which kernel takes rows of K logits: a thread a row up to 32 classes; the
-// registers of 8 or 32 lanes or of a block hold up to 32, 128 and 1024 words;
-// the ring takes longer rows.
+constexpr long long WARP_WORDS = 512;  // of a row that a warp can hold
+
+// Which kernel takes rows of K logits: a thread a row up to 32 classes; 4 to 32
+// lanes hold up to WARP_WORDS words in registers; the ring takes longer rows.
 template <typename T, int OP, bool ENT>
 static int run_rows(const RowsArgs &a, int &grid, cudaStream_t st) {
     constexpr int N = Vec<T>::N;
     if (a.K <= 8) return go_tile<T, OP, ENT, 8>(a, grid, st);
     if (a.K <= 16) return go_tile<T, OP, ENT, 16>(a, grid, st);
     if (a.K <= TILE_CLASSES) return go_tile<T, OP, ENT, TILE_CLASSES>(a, grid, st);
-    const long long words = (a.K + 2 * N - 2) / N;  // at most, whatever the alignment
-    if (words <= 32) return go_rows<T, OP, ENT, 8, 128, 4>(a, grid, st);
-    if (words <= 128) return go_rows<T, OP, ENT, 32, 128, 4>(a, grid, st);
-    if (words <= 1024) return go_rows<T, OP, ENT, 256, 256, 4>(a, grid, st);
-    // the ring wants the row and its gradient aligned alike
+    // all but the last kernel want the row and its gradient aligned alike
     const bool alike = OP == ROW_LOGP || ((reinterpret_cast<uintptr_t>(a.logits) - reinterpret_cast<uintptr_t>(a.grad)) % 16 == 0 &&
                                           (a.rows <= 1 || (a.stride - a.grad_stride) * (long long)sizeof(T) % 16 == 0));
+    const long long words = a.K / N;  // at most
+    if (alike && words <= WARP_WORDS) {
+        if (words <= 8) return go_rows<T, OP, ENT, 4, 2, 4>(a, grid, st);
+        if (words <= 16) return go_rows<T, OP, ENT, 8, 2, 8>(a, grid, st);
+        if (words <= 32) return go_rows<T, OP, ENT, 16, 2, 8>(a, grid, st);
+        if (words <= 64) return go_rows<T, OP, ENT, 32, 2, 8>(a, grid, st);
+        if (words <= 128) return go_rows<T, OP, ENT, 32, 4, 4>(a, grid, st);
+        if (words <= 256) return go_rows<T, OP, ENT, 32, 8, 2>(a, grid, st);
+        return go_rows<T, OP, ENT, 32, 16, 1>(a, grid, st);
+    }
     if (alike && a.K < (1ll << 30)) {
         if constexpr (OP == ROW_POLICY) {
             if (a.rows > 3 * sm_count() && a.K * (long long)sizeof(T) >= ONE_ROW) return go_ring<T, OP, ENT, 16, 1>(a, grid, st);
@@ -1398,8 +1543,9 @@ static int run_rows(const RowsArgs &a, int &grid, cudaStream_t st) {
         if (cl == 4) return go_ring<T, OP, ENT, 8, 4>(a, grid, st);
         return go_ring<T, OP, ENT, 8, 8>(a, grid, st);
     }
-    static int cache[64];
-    return launch_rows(k_rows_long<T, OP, ENT, 512>, a.rows, 512, 1, 0, cache, a, grid, st);
+    static int cache[2][64];
+    if (words <= WARP_WORDS) return launch_rows(k_rows_long<T, OP, ENT, 64>, a.rows, 64, 1, 0, cache[0], a, grid, st);
+    return launch_rows(k_rows_long<T, OP, ENT, 512>, a.rows, 512, 1, 0, cache[1], a, grid, st);
 }
 
 // `ent`: the call has an entropy (log-probs) or an entropy gradient.
