@@ -988,15 +988,14 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, unsigned b
                  : "memory");
 }
 
-// A ring for W warps that take words (8, or 16 in the one block of an SM), one
-// that copies and one that closes rows.
+// A ring for W warps that take words, one that copies and one that closes rows.
 template <int OP, int W>
 struct Ring {
     static constexpr int CONS = W * 32, NT = CONS + 64;
-    static constexpr int BLOCKS = W == 16 ? 1 : OP == ROW_GRAD ? 2 : 3;   // of an SM
-    static constexpr int LANE_WORDS = 4;                                  // of a lane in a stage
-    static constexpr int STAGE = CONS * LANE_WORDS;                       // words
-    static constexpr int STAGES = W == 16 || OP == ROW_GRAD ? 6 : 4;      // 192 KB of an SM under way
+    static constexpr int BLOCKS = W == 16 ? 1 : W == 4 ? 5 : OP == ROW_GRAD ? 2 : 3;         // of an SM
+    static constexpr int LANE_WORDS = 4;                                                     // of a lane in a stage
+    static constexpr int STAGE = CONS * LANE_WORDS;                                          // words
+    static constexpr int STAGES = W == 16 || (OP == ROW_GRAD && W == 8) ? 6 : 4;             // 160 or 192 KB of an SM
     static constexpr int SMEM = STAGES * STAGE * 16;
 };
 constexpr int RING_RECS = 8;  // at least the stages
@@ -1237,13 +1236,13 @@ __global__ void __launch_bounds__(Ring<OP, W>::NT, Ring<OP, W>::BLOCKS) k_rows_r
             if (rec.i < 0) break;
             if (OP != ROW_GRAD) {
                 Share<T, SENT> sh;
-                float x_y = 0.0f;
+                float x_y = 0.0f, x_end = -INFINITY;  // loaded now, needed at the row's end
                 if (rank == 0 && warp == 0) {  // the label's logit, and the elements outside the aligned words
                     const T *row = logits + rec.i * a.stride;
                     x_y = rec.y < K ? Vec<T>::to(row[rec.y]) : NAN;
                     const int tail = rec.head + rec.words * N;
                     const int at = lane < rec.head ? lane : lane >= 16 && tail + lane - 16 < K ? tail + lane - 16 : -1;
-                    if (at >= 0) sh.add_one(Vec<T>::to(row[at]), c);
+                    if (at >= 0) x_end = Vec<T>::to(row[at]);
                 }
                 for (int at = 0; at < rec.n; at += SW) {
                     read(w, slot, parity, rec.n - at);
@@ -1251,6 +1250,7 @@ __global__ void __launch_bounds__(Ring<OP, W>::NT, Ring<OP, W>::BLOCKS) k_rows_r
                     raise_floor(w);
                     sh.template add<LW>(w, c);
                 }
+                sh.add_one(x_end, c);
                 RowSum sum = lanes_join<32, SENT>(sh.sum(), HALF ? 1.0f : c);
                 if (lost) sum.s = NAN;
                 if (OP == ROW_LOGP && k >= 2) bar_wait(&closed[k & 1], ((k >> 1) - 1) & 1, lost);
@@ -1501,6 +1501,12 @@ static int go_ring(const RowsArgs &a, int &grid, cudaStream_t st) {
 // (65536 bf16 classes: 205 against 239 us for 4096 rows; 50000: 197 against 164).
 constexpr long long ONE_ROW = 112 << 10;
 
+// Words of a row up to which four warps share it and five rows an SM: a row's
+// joining and closing then waits beside four others (policy step of 16000 x 8000
+// bf16 131 us against 163 with eight warps; of 4000 x 32000, past it, 113 against
+// 107).
+constexpr long long FOUR_WARPS = 2048;
+
 template <typename T, int OP, bool ENT, int KM>
 static int go_tile(const RowsArgs &a, int &grid, cudaStream_t st) {
     static int cache[64];
@@ -1535,6 +1541,7 @@ static int run_rows(const RowsArgs &a, int &grid, cudaStream_t st) {
         if constexpr (OP == ROW_POLICY) {
             if (a.rows > 3 * sm_count() && a.K * (long long)sizeof(T) >= ONE_ROW) return go_ring<T, OP, ENT, 16, 1>(a, grid, st);
         }
+        if (words <= FOUR_WARPS && a.rows > 3 * sm_count()) return go_ring<T, OP, ENT, 4, 1>(a, grid, st);
         int cl = 1;
         // few rows: more blocks to a row, while the SMs are not all taken
         while (cl < 8 && a.rows * cl * 2 <= sm_count()) cl *= 2;
