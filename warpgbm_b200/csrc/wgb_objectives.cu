@@ -252,7 +252,7 @@ __device__ __forceinline__ void quad_seqs(const Idx &off, long long S, long long
 }
 
 // Four neighbouring values from t on, those past the end as `none`; `whole`:
-// the array may be read 16 (mask: 4) bytes at a time.
+// the array may be read in words.
 __device__ __forceinline__ void quad_load(const float *p, long long t, long long T, bool whole, float none, float (&v)[4]) {
     if (whole && t + 4 <= T) {
         const float4 u = *reinterpret_cast<const float4 *>(p + t);
@@ -284,97 +284,109 @@ __device__ __forceinline__ void quad_mask(const uint8_t *p, long long t, long lo
     }
 }
 
-// Calls add(q, v, n) with the sums of v and n over neighbouring lanes of one
-// sequence q >= 0; every lane of a warp calls it.
-template <typename F>
-__device__ __forceinline__ void warp_by_seq(long long q, double v, int n, F add) {
-    const int lane = threadIdx.x & 31;
-    const unsigned full = 0xffffffffu;
-    const long long prev = __shfl_up_sync(full, q, 1);
-    const unsigned heads = __ballot_sync(full, lane == 0 || prev != q);
-    const int head = 31 - __clz(heads & (0xffffffffu >> (31 - lane)));
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {  // inclusive sums from each run's first lane
-        const double w = __shfl_up_sync(full, v, o);
-        const int k = __shfl_up_sync(full, n, o);
-        if (lane - o >= head) {
-            v += w;
-            n += k;
-        }
-    }
-    const bool last = lane == 31 || ((heads >> (lane + 1)) & 1u);
-    if (last && q >= 0 && n) add(q, v, n);
-}
-
-// Sums of a warp's range by sequence: fetch(t, keep, v) gives the four tokens
-// from t on whether they are kept and their values; add(q, v, n), called by one
-// lane, takes what the range has of sequence q.  `start` gets the range's first
-// place, for the parts to come.
-template <bool VALUES, typename FETCH, typename ADD>
+// Sums of a warp's range by sequence.  A lane has PER neighbouring tokens of a
+// chunk of 32 PER: fetch(t) gives the tokens from t on, as `keep` bits and, with
+// VALUES, `v`.  The chunk's sums up to each lane's first token are scanned, and
+// lane l finds the sum up to the l-th boundary of the chunk: a sequence's part is
+// the difference of two, whatever the number of sequences.  add(q, v, n), by one
+// lane each, takes what the range has of sequence q.  `start` gets the range's
+// first place, for the parts to come.
+template <bool VALUES, int PER>
+struct Tokens {
+    unsigned keep;
+    float v[VALUES ? PER : 1];
+};
+template <bool VALUES, int PER, typename FETCH, typename ADD>
 __device__ __forceinline__ void range_by_seq(const Idx &off, long long S, const Range &r, Place *start, FETCH fetch, ADD add) {
     if (r.a >= r.b) return;
+    constexpr int CHUNK = 32 * PER;
+    constexpr unsigned FULL = 0xffffffffu;
     const int lane = threadIdx.x & 31;
+    Tokens<VALUES, PER> more = fetch(r.a + lane * PER);
     Place at;
     at.find(off, S, 0, r.a);
     if (lane == 0) start[warp_index()] = at;
-    double sum = 0.0;  // of the sequence that the warp is in
+    long long q = at.q;                // sequence that the warp is in, -1 and S as in Place
+    double sum = 0.0;                  // of it, by lane
     int count = 0;
-    auto flush = [&]() {
-        const double v = VALUES ? warp_sum(sum) : 0.0;
-        const int n = warp_sum(count);
-        if (lane == 0 && n && at.valid(S)) add(at.q, v, n);
-        sum = 0.0;
-        count = 0;
+    long long b = LLONG_MAX;           // lane l: the end of sequence q + l
+    auto ends = [&]() { b = q + 1 + lane <= S ? off.at(q + 1 + lane) : LLONG_MAX; };
+    ends();
+    auto give = [&](long long to, double v, int n) {
+        if (n && to >= 0 && to < S) add(to, v, n);
     };
-    bool more[4];
-    float ahead[4];
-    fetch(r.a + lane * 4, more, ahead);  // says no past the last token, where a range may end
-    for (long long t0 = r.a; t0 < r.b; t0 += STEP) {
-        const long long t1 = t0 + STEP < r.b ? t0 + STEP : r.b, t = t0 + lane * 4;
-        bool keep[4];
-        float v[4];
+    for (long long t0 = r.a; t0 < r.b; t0 += CHUNK) {
+        const long long t1 = t0 + CHUNK < r.b ? t0 + CHUNK : r.b;
+        const Tokens<VALUES, PER> x = more;
+        if (t1 < r.b) more = fetch(t0 + CHUNK + lane * PER);
+        // only tokens below t1: a range may end inside a chunk
+        const long long left = t1 - (t0 + lane * PER);
+        const unsigned keep = left >= PER ? x.keep : left > 0 ? x.keep & ((1u << left) - 1u) : 0u;
+        double own = 0.0;
+        if (VALUES) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            keep[j] = more[j];
-            v[j] = ahead[j];
+            for (int j = 0; j < PER; ++j) own += keep >> j & 1u ? (double)x.v[j] : 0.0;
         }
-        if (t1 < r.b) fetch(t + STEP, more, ahead);
-        if (at.end >= t1 && at.end > t0) {  // one sequence
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (VALUES) sum += keep[j] ? (double)v[j] : 0.0;
-                count += keep[j];
-            }
+        const int own_n = __popc(keep);
+        if (__shfl_sync(FULL, b, 0) >= t1) {  // one sequence
+            sum += own;
+            count += own_n;
             continue;
         }
-        if (many_seqs(off, S, at, t1)) {
-            flush();
-            const long long first = at.q;
-            at.find(off, S, at.q + 1, t1 - 1);
-            long long q[4];
-            quad_seqs(off, S, first, at.q, t, q);
+        double scan = own;  // up to and with this lane, then in front of it
+        int scan_n = own_n;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) warp_by_seq(q[j], VALUES && keep[j] ? (double)v[j] : 0.0, keep[j], add);
-            continue;
-        }
-        const int n = (int)(t1 - t0);
-        for (int from = 0; from < n;) {
-            if (at.end <= t0 + from) {
-                flush();
-                at.next(off, S, t0 + from);
-                if (at.end <= t0 + from) break;  // offsets that do not rise
+        for (int o = 1; o < 32; o <<= 1) {
+            const double w = VALUES ? __shfl_up_sync(FULL, scan, o) : 0.0;
+            const int k = __shfl_up_sync(FULL, scan_n, o);
+            if (lane >= o) {
+                scan += w;
+                scan_n += k;
             }
-            const int to = at.end < t1 ? (int)(at.end - t0) : n;
+        }
+        const double all = VALUES ? __shfl_sync(FULL, scan, 31) : 0.0;
+        const int all_n = __shfl_sync(FULL, scan_n, 31);
+        scan -= own;
+        scan_n -= own_n;
+        // what the sequence q had before this chunk
+        double before = VALUES ? warp_sum(sum) : 0.0;
+        int before_n = warp_sum(count);
+        double given = 0.0;  // of this chunk, to sequences that have ended
+        int given_n = 0;
+        for (;;) {
+            // boundaries in this chunk, in the lanes from 0 on
+            const unsigned in = __ballot_sync(FULL, b < t1);
+            const int nb = __popc(in);
+            if (!nb) break;
+            const int rel = b > t0 ? b < t1 ? (int)(b - t0) : CHUNK - 1 : 0;
+            const int from = rel / PER, j = rel % PER;
+            double part = 0.0;
+            if (VALUES) {
+                part = __shfl_sync(FULL, scan, from);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (keep[j] && lane * 4 + j >= from && lane * 4 + j < to) {
-                    if (VALUES) sum += (double)v[j];
-                    ++count;
+                for (int k = 0; k < PER - 1; ++k) {  // the tokens of that lane before the boundary
+                    const float v = __shfl_sync(FULL, keep >> k & 1u ? x.v[k] : 0.0f, from);
+                    if (k < j) part += (double)v;
                 }
-            from = to;
+            }
+            const int part_n = __shfl_sync(FULL, scan_n, from) + __popc(__shfl_sync(FULL, keep, from) & ((1u << j) - 1u));
+            const double last = __shfl_up_sync(FULL, part, 1);
+            const int last_n = __shfl_up_sync(FULL, part_n, 1);
+            if (lane < nb)
+                give(q + lane, lane ? part - last : part - given + before, lane ? part_n - last_n : part_n - given_n + before_n);
+            before = 0.0;
+            before_n = 0;
+            given = __shfl_sync(FULL, part, nb - 1);
+            given_n = __shfl_sync(FULL, part_n, nb - 1);
+            q += nb;
+            ends();
         }
+        sum = lane == 0 ? all - given : 0.0;
+        count = lane == 0 ? all_n - given_n : 0;
     }
-    flush();
+    sum = VALUES ? warp_sum(sum) : 0.0;
+    count = warp_sum(count);
+    if (lane == 0) give(q, sum, count);
 }
 
 // --------------------------------------------------------- preference --
@@ -439,7 +451,7 @@ struct PrefArgs {
     unsigned long long *count;  // kept tokens by sequence (ragged)
     float *diff;                // logp - ref by row (not ragged, with a reference)
     Place *places;              // where each warp's range of tokens starts (ragged)
-    bool whole, whole_mask;     // arrays on 16-byte (mask: 4-byte) boundaries
+    bool whole, whole_mask;     // arrays and mask on 16-byte boundaries
     int n_top, n_partial;       // blocks that gave a weight, a share of the loss
     Cut cut;
 };
@@ -506,16 +518,22 @@ __device__ __forceinline__ void pref_start(const PrefArgs &a) {
 }
 // Sequence sums of logp - ref over the kept tokens.
 __device__ __forceinline__ void pref_sums(const PrefArgs &a) {
-    range_by_seq<true>(a.off, a.S, a.cut.range(), a.places,
-        [&](long long t, bool (&keep)[4], float (&v)[4]) {
+    range_by_seq<true, 4>(a.off, a.S, a.cut.range(), a.places,
+        [&](long long t) {
+            Tokens<true, 4> x;
+            bool keep[4];
             quad_mask(a.mask, t, a.T, a.whole_mask, keep);
-            quad_load(a.logp, t, a.T, a.whole, 0.0f, v);
+            quad_load(a.logp, t, a.T, a.whole, 0.0f, x.v);
             if (a.ref) {
                 float r[4];
                 quad_load(a.ref, t, a.T, a.whole, 0.0f, r);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] -= r[j];
+                for (int j = 0; j < 4; ++j) x.v[j] -= r[j];
             }
+            x.keep = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x.keep |= (unsigned)keep[j] << j;
+            return x;
         },
         [&](long long q, double v, int n) {
             a.scores.add(q, v);
@@ -768,19 +786,29 @@ struct CountArgs {
 __device__ __forceinline__ void policy_count(const CountArgs &a, double *scratch) {
     long long kept = 0, full = 0;
     const Range r = a.cut.range();
-    auto fetch = [&](long long t, bool (&keep)[4], float (&v)[4]) {
-        quad_mask(a.mask, t, a.T, a.whole_mask, keep);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (a.labels.p) keep[j] = keep[j] && a.labels.at(t + j) >= 0;  // keep: t + j < T
-            v[j] = 0.0f;
-        }
-    };
     if (a.off.p) {
-        range_by_seq<false>(a.off, a.S, r, a.cnt.places, fetch, [&](long long q, double, int n) {
-            if (a.by_sequence) full += atomicAdd(a.cnt.count + q, (unsigned long long)n) == 0;
-            kept += n;
-        });
+        range_by_seq<false, 16>(a.off, a.S, r, a.cnt.places,
+            [&](long long t) {
+                Tokens<false, 16> x;
+                x.keep = 0;
+                if (!a.labels.p && a.mask && a.whole_mask && t + 16 <= a.T) {
+                    const uint4 m = *reinterpret_cast<const uint4 *>(a.mask + t);
+                    const unsigned w[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)  // a bit for each byte that is not zero
+                        x.keep |= (((__vcmpne4(w[i], 0u) & 0x08040201u) * 0x01010101u) >> 24 & 15u) << (4 * i);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (t + j < a.T && (!a.mask || a.mask[t + j]) && (!a.labels.p || a.labels.at(t + j) >= 0))
+                            x.keep |= 1u << j;
+                }
+                return x;
+            },
+            [&](long long q, double, int n) {
+                if (a.by_sequence) full += atomicAdd(a.cnt.count + q, (unsigned long long)n) == 0;
+                kept += n;
+            });
         if (a.cnt.ids && r.a < r.b) {
             __syncwarp();
             const long long first = a.cnt.places[warp_index()].q;
@@ -797,10 +825,9 @@ __device__ __forceinline__ void policy_count(const CountArgs &a, double *scratch
     } else {
         for (long long t = r.a + (threadIdx.x & 31) * 4; t < r.b; t += STEP) {
             bool keep[4];
-            float none[4];
-            fetch(t, keep, none);
+            quad_mask(a.mask, t, a.T, a.whole_mask, keep);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) kept += keep[j] && t + j < r.b;
+            for (int j = 0; j < 4; ++j) kept += keep[j] && (!a.labels.p || a.labels.at(t + j) >= 0);
         }
     }
     // whole numbers below 2^53: exact as double
@@ -1054,7 +1081,6 @@ static int part_grid(long long items, int each) { return grid_of(items, each, sm
 static int walk_grid(long long tokens) { return grid_of(tokens, GRID_THREADS / 32 * STEP, sm_count() * 3); }
 static long long places_bytes() { return (long long)sm_count() * MAX_BLOCKS_PER_SM * (GRID_THREADS / 32) * sizeof(Place); }
 static bool on16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
-static bool on4(const void *p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 
 }  // namespace wgb
 
@@ -1146,7 +1172,7 @@ extern "C" int wgb_preference_loss(const float *logp, const float *ref_logp, int
     a.diff = w.diff;
     a.places = w.places;
     a.whole = on16(logp) && on16(ref_logp) && on16(grad_logp);
-    a.whole_mask = on4(mask);
+    a.whole_mask = on16(mask);
     cudaStream_t st = as_stream(stream);
     const dim3 nt(GRID_THREADS);
     // a pair costs about as much as four tokens, a sequence as two
@@ -1221,7 +1247,7 @@ static int policy_rule(const PolicyArgs &a, const float *ref, long long tokens, 
 
 static CountArgs count_args(const PolicyWs &w, const uint8_t *mask, Idx labels, long long tokens, Idx off,
                             long long sequences, const PolicyRule &rule) {
-    return CountArgs{mask,   labels, tokens, off, sequences, rule.by_sequence != 0, on4(mask),
+    return CountArgs{mask,   labels, tokens, off, sequences, rule.by_sequence != 0, on16(mask),
                      w.cnt,  rule.by_sequence ? w.zero_bytes : 32};
 }
 // The kernels that count, for a kernel to follow.
