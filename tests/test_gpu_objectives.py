@@ -749,3 +749,64 @@ def test_many_rows(obj, n, k, dtype):
     for i in ok.nonzero()[:: max(1, w // 5), 0].tolist():
         one = obj.label_logprobs(x[i:i + 1].clone(), y[i:i + 1])
         assert abs(float(one.logp[0]) - float(r.logp[i])) < tol
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,k", [(600, 70001), (460, 60000), (1500, 8200), (3000, 700), (4000, 70)])
+def test_policy_rows_out_of_the_ordinary_among_many(obj, n, k, dtype):
+    """Rows left out, masked whole, with the lowest value throughout or with NaN, between plain ones, in place."""
+    x = make_logits(k, n, k, dtype, scale=2.0).clone()
+    y = make_labels(k, n, k)
+    y[5::7] = -1
+    empty, lowest, nan = n // 3, n // 3 + 1, n // 2
+    y[empty], y[lowest], y[nan] = 1, 2, 3
+    x[empty] = -math.inf
+    x[lowest] = LOWEST[dtype]
+    x[nan, k - 1] = math.nan
+    base = obj.label_logprobs(x, y, entropy=True)
+    old = torch.where(torch.isfinite(base.logp), base.logp, torch.zeros_like(base.logp)) - ratios(3, n)
+    adv = torch.randn(n, device="cuda", generator=gen(4))
+    want_logp = -math.log(k)
+    assert float(base.logp[empty]) == -math.inf and abs(float(base.logp[lowest]) - want_logp) < 1e-4
+    mask = torch.ones(n, dtype=torch.bool, device="cuda")
+    mask[[empty, nan]] = False
+    a = obj.policy_loss_logits(x, y, old, adv, mask=mask, entropy_coef=0.05, grad_scale=float(n))
+    parts = obj.policy_loss(base.logp.nan_to_num(0, 0, 0), old, adv, mask=mask & (y >= 0))
+    assert abs(float(a.policy) - float(parts.policy)) < 1e-5 * (1 + abs(float(parts.policy)))
+    kept = mask & (y >= 0)
+    w = 1.0 / float(kept.sum())
+    ent = float((base.entropy[kept].double()).sum() * w)
+    assert abs(float(a.entropy) - ent) < 1e-5 * (1 + ent)
+    assert torch.equal(a.logp[~kept], torch.zeros_like(a.logp[~kept])) and not a.grad_logits[~kept].any()
+    assert torch.isfinite(a.grad_logits).all()
+    # the uniform row: p = 1/k in every place, g (1[y] - 1/k), no entropy gradient
+    g = float(parts.grad_logp[lowest]) * n
+    row = f64(a.grad_logits[lowest])
+    want = np.full(k, -g / k)
+    want[2] += g
+    assert np.abs(row - want).max() < (EPS[dtype] * 1.01 + 1e-4) * abs(g) / 1 + TINY[dtype]
+    # rows of the gradient sum to nothing but rounding
+    sums = a.grad_logits.double().sum(1)
+    size = a.grad_logits.double().abs().sum(1)
+    assert float((sums.abs() - (EPS[dtype] * 2 + 1e-4) * size - k * TINY[dtype]).max()) <= 1e-12
+    b = obj.policy_loss_logits(x, y, old, adv, mask=mask, entropy_coef=0.05, grad_scale=float(n), out=x)
+    assert torch.equal(b.grad_logits, a.grad_logits) and torch.equal(b.loss, a.loss) and torch.equal(b.logp, a.logp)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,k", [(40, 20), (40, 300), (20, 9000)])
+def test_gradients_beside_the_logits_and_unlike_aligned(obj, n, k, dtype):
+    """Logits and gradient as columns of one buffer, at every alignment to one another."""
+    for shift in (0, 1, 3):
+        buf = torch.randn(n, 2 * k + 16, device="cuda", generator=gen(k)).to(dtype)
+        x, out = buf[:, :k], buf[:, k + 8 + shift:2 * k + 8 + shift]
+        y = make_labels(k, n, k)
+        old, adv = torch.full((n,), -3.0, device="cuda"), torch.randn(n, device="cuda", generator=gen(4))
+        keep = x.clone()
+        want = obj.policy_loss_logits(keep, y, old, adv, entropy_coef=0.1)
+        got = obj.policy_loss_logits(x, y, old, adv, entropy_coef=0.1, out=out)
+        assert torch.equal(x, keep) and got.grad_logits.data_ptr() == out.data_ptr()
+        tol = row_tol(f64(keep)).max()
+        err = (got.grad_logits.double() - want.grad_logits.double()).abs()
+        bound = 2 * EPS[dtype] * 1.01 * want.grad_logits.double().abs() + 8 * tol * float(adv.abs().max()) / n + TINY[dtype]
+        assert float((err - bound).max()) <= 0

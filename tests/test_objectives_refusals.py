@@ -171,3 +171,11 @@ def test_workspace_sizes_hold_what_they_name():
     assert L.wgb_preference_ws_bytes(0, 0) > 0
     assert L.wgb_preference_ws_bytes(1000, 1) > L.wgb_preference_ws_bytes(1000, 0) >= 24 * 1000
     assert L.wgb_policy_ws_bytes(1000, 10, 1) >= L.wgb_policy_ws_bytes(1000, 10, 0) + 4000
+
+
+def test_columns_of_one_buffer_do_not_overlap():
+    buf = cuda(4, 8)
+    x, y, v = buf[:, :3], cuda(4, dtype=torch.int64), cuda(4)
+    with pytest.raises(ValueError, match="logits itself or not overlap"):
+        obj.label_logprobs_grad(x, y, v, v, out=buf[:, 2:5])
+    assert obj._grad_like(x, 8, buf[:, 3:6])[1] == 8  # side by side: taken

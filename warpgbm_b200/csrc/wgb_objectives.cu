@@ -518,21 +518,24 @@ __device__ __forceinline__ void pref_start(const PrefArgs &a) {
 }
 // Sequence sums of logp - ref over the kept tokens.
 __device__ __forceinline__ void pref_sums(const PrefArgs &a) {
-    range_by_seq<true, 4>(a.off, a.S, a.cut.range(), a.places,
-        [&](long long t) {
-            Tokens<true, 4> x;
-            bool keep[4];
-            quad_mask(a.mask, t, a.T, a.whole_mask, keep);
-            quad_load(a.logp, t, a.T, a.whole, 0.0f, x.v);
-            if (a.ref) {
-                float r[4];
-                quad_load(a.ref, t, a.T, a.whole, 0.0f, r);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x.v[j] -= r[j];
-            }
+    range_by_seq<true, 8>(a.off, a.S, a.cut.range(), a.places,
+        [&](long long t0) {
+            Tokens<true, 8> x;
             x.keep = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x.keep |= (unsigned)keep[j] << j;
+            for (int i = 0; i < 8; i += 4) {
+                const long long t = t0 + i;
+                bool keep[4];
+                float v[4], r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                quad_mask(a.mask, t, a.T, a.whole_mask, keep);
+                quad_load(a.logp, t, a.T, a.whole, 0.0f, v);
+                if (a.ref) quad_load(a.ref, t, a.T, a.whole, 0.0f, r);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    x.v[i + j] = v[j] - r[j];
+                    x.keep |= (unsigned)keep[j] << (i + j);
+                }
+            }
             return x;
         },
         [&](long long q, double v, int n) {
@@ -588,41 +591,64 @@ __device__ __forceinline__ void pref_pairs(const PrefArgs &a, double *scratch) {
     total = block_sum(total, scratch);
     if (threadIdx.x == 0) a.partial[blockIdx.x] = total;
 }
-// The loss, and the gradient of every token: its sequence's, where it is kept.
+// The loss, from the blocks' shares.
 template <int NT>
-__device__ __forceinline__ void pref_grad(const PrefArgs &a, double *scratch) {
-    const bool bounded = a.rule.kind != 2;
-    const GridSums grid_sums = pref_grid_sums(a);
-    const double inv = a.P ? 1.0 / (double)a.P : 0.0;
+__device__ __forceinline__ void pref_loss(const PrefArgs &a, double inv, double *scratch) {
     if (blockIdx.x == 0) {
         double v = 0.0;
         for (int i = threadIdx.x; i < a.n_partial; i += NT) v += a.partial[i];
         v = block_sum(v, scratch);
         if (threadIdx.x == 0) *a.loss = (float)(v * inv);
     }
+}
+// The gradient of every row, from its pairs.
+template <int NT>
+__device__ __forceinline__ void pref_row_grad(const PrefArgs &a, double *scratch) {
+    const bool bounded = a.rule.kind != 2;
+    const GridSums grid_sums = pref_grid_sums(a);
+    const double inv = a.P ? 1.0 / (double)a.P : 0.0;
+    pref_loss<NT>(a, inv, scratch);
+    const Range range = a.cut.range();
+    for (long long t = range.a + (threadIdx.x & 31) * 4; t < range.b; t += STEP) {
+        float g[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            g[j] = t + j < a.T ? (float)((bounded ? grid_sums.value(t + j) : a.grads.value(t + j)) * inv) : 0.0f;
+        quad_store(a.grad, t, a.T, a.whole, g);
+    }
+}
+// The gradient of every token: its sequence's, where it is kept.
+template <int NT>
+__device__ __forceinline__ void pref_grad(const PrefArgs &a, double *scratch) {
+    const bool bounded = a.rule.kind != 2;
+    const GridSums grid_sums = pref_grid_sums(a);
+    const double inv = a.P ? 1.0 / (double)a.P : 0.0;
+    pref_loss<NT>(a, inv, scratch);
     auto grad_of = [&](long long q) {
         const double v = (bounded ? grid_sums.value(q) : a.grads.value(q)) * inv;
         return (float)(a.rule.average && a.count[q] ? v / (double)a.count[q] : v);
     };
     const Range range = a.cut.range();
     const int lane = threadIdx.x & 31;
-    if (!a.off.p) {
-        for (long long t = range.a + lane * 4; t < range.b; t += STEP) {
-            float g[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) g[j] = t + j < a.T ? grad_of(t + j) : 0.0f;
-            quad_store(a.grad, t, a.T, a.whole, g);
-        }
-        return;
-    }
     if (range.a >= range.b) return;
     Place at = a.places[warp_index()];
-    float of = at.valid(a.S) ? grad_of(at.q) : 0.0f;
+    float of = 0.0f, held = 0.0f;  // of the sequence that the warp is in, and of the next, loaded ahead
+    long long held_q = -2;
+    auto enter = [&]() {
+        of = !at.valid(a.S) ? 0.0f : at.q == held_q ? held : grad_of(at.q);
+        held_q = at.q + 1;
+        held = held_q >= 0 && held_q < a.S ? grad_of(held_q) : 0.0f;
+    };
+    enter();
+    bool more[4];
+    quad_mask(a.mask, range.a + lane * 4, a.T, a.whole_mask, more);
     for (long long t0 = range.a; t0 < range.b; t0 += STEP) {
         const long long t1 = t0 + STEP < range.b ? t0 + STEP : range.b, t = t0 + lane * 4;
         bool keep[4];
         float g[4];
-        quad_mask(a.mask, t, a.T, a.whole_mask, keep);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) keep[j] = more[j];
+        if (t1 < range.b) quad_mask(a.mask, t + STEP, a.T, a.whole_mask, more);
         if (many_seqs(a.off, a.S, at, t1)) {
             const long long first = at.q;
             at.find(a.off, a.S, at.q + 1, t1 - 1);
@@ -630,14 +656,14 @@ __device__ __forceinline__ void pref_grad(const PrefArgs &a, double *scratch) {
             quad_seqs(a.off, a.S, first, at.q, t, q);
 #pragma unroll
             for (int j = 0; j < 4; ++j) g[j] = q[j] < 0 ? 0.0f : j > 0 && q[j] == q[j - 1] ? g[j - 1] : grad_of(q[j]);
-            of = at.valid(a.S) ? grad_of(at.q) : 0.0f;
+            enter();
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) g[j] = of;
             while (at.end < t1) {
                 const long long from = at.end > t0 ? at.end : t0;
                 at.next(a.off, a.S, from);
-                of = at.valid(a.S) ? grad_of(at.q) : 0.0f;
+                enter();
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (t + j >= from) g[j] = of;
@@ -659,6 +685,7 @@ __global__ void __launch_bounds__(GRID_THREADS) k_pref_part(const __grid_constan
     if (PART == 2) pref_pairs<true, GRID_THREADS>(a, scratch);
     if (PART == 4) pref_pairs<false, GRID_THREADS>(a, scratch);
     if (PART == 3) pref_grad<GRID_THREADS>(a, scratch);
+    if (PART == 5) pref_row_grad<GRID_THREADS>(a, scratch);
 }
 __global__ void __launch_bounds__(BLOCK_THREADS) k_pref_block(const __grid_constant__ PrefArgs a) {
     __shared__ double scratch[33];
@@ -672,7 +699,8 @@ __global__ void __launch_bounds__(BLOCK_THREADS) k_pref_block(const __grid_const
     if (a.off.p) pref_pairs<true, BLOCK_THREADS>(a, scratch);
     else pref_pairs<false, BLOCK_THREADS>(a, scratch);
     __syncthreads();
-    pref_grad<BLOCK_THREADS>(a, scratch);
+    if (a.off.p) pref_grad<BLOCK_THREADS>(a, scratch);
+    else pref_row_grad<BLOCK_THREADS>(a, scratch);
 }
 
 // ------------------------------------------------------------- policy --
@@ -1190,7 +1218,8 @@ extern "C" int wgb_preference_loss(const float *logp, const float *ref_logp, int
     if (offsets) WGB_PDL("k_pref_part", k_pref_part<1>, dim3(tok), nt, 0, st, a);
     if (offsets) WGB_PDL("k_pref_part", k_pref_part<2>, dim3(a.n_partial), nt, 0, st, a);
     else WGB_PDL("k_pref_part", k_pref_part<4>, dim3(a.n_partial), nt, 0, st, a);
-    WGB_PDL("k_pref_part", k_pref_part<3>, dim3(tok), nt, 0, st, a);
+    if (offsets) WGB_PDL("k_pref_part", k_pref_part<3>, dim3(tok), nt, 0, st, a);
+    else WGB_PDL("k_pref_part", k_pref_part<5>, dim3(tok), nt, 0, st, a);
     return WGB_OK;
 }
 

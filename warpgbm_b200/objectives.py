@@ -137,7 +137,9 @@ def _grad_like(logits, stride, out):
     a, b, size = logits.data_ptr(), out.data_ptr(), logits.element_size()
     if n and not (a == b and stride == out_stride) and \
             a < b + ((n - 1) * out_stride + k) * size and b < a + ((n - 1) * stride + k) * size:
-        raise ValueError("out must be logits itself or not overlap it")
+        apart = (b - a) % (stride * size)  # columns of one buffer, side by side
+        if n > 1 and (stride != out_stride or apart < k * size or apart + k * size > stride * size) or n == 1:
+            raise ValueError("out must be logits itself or not overlap it")
     return out, out_stride
 
 
