@@ -22,6 +22,7 @@ NVCC_FLAGS = [
     "-O3", "-lineinfo", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-pthread", "-shared",
     "-Xptxas", "-warn-spills",
+    "--split-compile=0",  # as many threads as there are cores: the kernels come in many types
 ]
 
 

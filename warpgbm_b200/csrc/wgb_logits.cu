@@ -526,7 +526,7 @@ __device__ __forceinline__ void word_emit(const RowWords<T, J> &rw, T *out, J q,
 }
 
 // --------------------------------------------------------- rows, by call --
-enum RowOp { ROW_LOGP, ROW_GRAD, ROW_POLICY };
+enum { ROW_LOGP, ROW_GRAD, ROW_POLICY };
 
 struct RowsArgs {
     const void *logits;
@@ -735,7 +735,9 @@ __device__ __noinline__ float4 careful_row(const RowsArgs &a, long long i, float
 // once (its scalars, its logarithm, the loss) is done by a lane of its own for
 // all rows of the warp together: repeated by all lanes of a row it took most of
 // the time of short rows.  ROW_POLICY keeps the words in shared memory (8 KB a
-// warp) until the gradient, so that a row is read once.
+// warp) until the gradient, so that a row is read once.  Bound by instruction
+// issue (0.5 to 0.65 of the slots): the policy step of 500000 x 255 bf16 takes 202
+// us (HBM alone 80), of 32000 x 4096 140 (80), log-probs of 32000 x 4000 49 (39).
 constexpr int WARP_NT = 128;
 template <typename T, int GL, int U, int B>
 struct Batch {
@@ -1034,6 +1036,11 @@ __device__ __forceinline__ RowRec row_rec(const T *row, int K, long long i, int 
 // 4096 x 131072 bf16 against 390: the blocks of a cluster wait for one another
 // twice a row.
 //
+// Measured at 4096 x 131072 bf16 (1.07 GB): log-probs 161 us, HBM at its copy
+// rate; policy step 388 us, 0.84 of it, the exponential unit busy for 0.63 of the
+// time (two a logit).  Their gradient alone at 2047 x 50001 f16: 0.9 of the copy
+// rate.
+//
 // In place a gradient is written only after the whole row is read: the row's own
 // words, its ends and the label's logit all go into what a warp puts.
 //
@@ -1311,7 +1318,9 @@ __global__ void __launch_bounds__(Ring<OP, W>::NT, Ring<OP, W>::BLOCKS) k_rows_r
 // words whatever the number of classes; a thread then holds its row in KM
 // registers.  Threads t and t + 32 / g (g the power of two in a row's 4-byte
 // words) would meet in the same bank, so each such group starts its row at an
-// element of its own.
+// element of its own.  Bound by instruction issue (0.65 of the slots, a third of
+// them for what a row does once): 1000000 x 10 f32 log-probs 16 us, policy step 42
+// (HBM alone 16).
 constexpr int TILE_ROWS = 128;
 constexpr int TILE_CLASSES = 32;
 
@@ -1542,26 +1551,29 @@ static int run_rows(const RowsArgs &a, int &grid, cudaStream_t st) {
             if (a.rows > 3 * sm_count() && a.K * (long long)sizeof(T) >= ONE_ROW) return go_ring<T, OP, ENT, 16, 1>(a, grid, st);
         }
         if (words <= FOUR_WARPS && a.rows > 3 * sm_count()) return go_ring<T, OP, ENT, 4, 1>(a, grid, st);
-        int cl = 1;
-        // few rows: more blocks to a row, while the SMs are not all taken
-        while (cl < 8 && a.rows * cl * 2 <= sm_count()) cl *= 2;
-        if (cl == 1) return go_ring<T, OP, ENT, 8, 1>(a, grid, st);
-        if (cl == 2) return go_ring<T, OP, ENT, 8, 2>(a, grid, st);
-        if (cl == 4) return go_ring<T, OP, ENT, 8, 4>(a, grid, st);
-        return go_ring<T, OP, ENT, 8, 8>(a, grid, st);
+        // few rows: as many blocks to a row as the SMs allow
+        if (a.rows * 8 <= sm_count()) return go_ring<T, OP, ENT, 8, 8>(a, grid, st);
+        if (a.rows * 4 <= sm_count()) return go_ring<T, OP, ENT, 8, 4>(a, grid, st);
+        return go_ring<T, OP, ENT, 8, 1>(a, grid, st);
     }
-    static int cache[2][64];
-    if (words <= WARP_WORDS) return launch_rows(k_rows_long<T, OP, ENT, 64>, a.rows, 64, 1, 0, cache[0], a, grid, st);
-    return launch_rows(k_rows_long<T, OP, ENT, 512>, a.rows, 512, 1, 0, cache[1], a, grid, st);
+    static int cache[64];
+    return launch_rows(k_rows_long<T, OP, ENT, 256>, a.rows, 256, 1, 0, cache, a, grid, st);
 }
 
-// `ent`: the call has an entropy (log-probs) or an entropy gradient.
+// `ent`: the call has an entropy (log-probs) or an entropy gradient; the policy
+// step always has one.
+template <typename T, int OP>
+static int run_ent(bool ent, const RowsArgs &a, int &grid, cudaStream_t st) {
+    if constexpr (OP != ROW_POLICY) {
+        if (!ent) return run_rows<T, OP, false>(a, grid, st);
+    }
+    return run_rows<T, OP, true>(a, grid, st);
+}
 template <int OP>
 static int run_typed(int dtype, bool ent, const RowsArgs &a, int &grid, cudaStream_t st) {
-    if (dtype == 0) return ent ? run_rows<float, OP, true>(a, grid, st) : run_rows<float, OP, false>(a, grid, st);
-    if (dtype == 1)
-        return ent ? run_rows<__nv_bfloat16, OP, true>(a, grid, st) : run_rows<__nv_bfloat16, OP, false>(a, grid, st);
-    return ent ? run_rows<__half, OP, true>(a, grid, st) : run_rows<__half, OP, false>(a, grid, st);
+    if (dtype == 0) return run_ent<float, OP>(ent, a, grid, st);
+    if (dtype == 1) return run_ent<__nv_bfloat16, OP>(ent, a, grid, st);
+    return run_ent<__half, OP>(ent, a, grid, st);
 }
 
 }  // namespace wgb
