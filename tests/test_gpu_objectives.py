@@ -793,6 +793,63 @@ def test_policy_rows_out_of_the_ordinary_among_many(obj, n, k, dtype):
     assert torch.equal(b.grad_logits, a.grad_logits) and torch.equal(b.loss, a.loss) and torch.equal(b.logp, a.logp)
 
 
+@pytest.mark.parametrize("n,k,dtype", [(460, 80001, torch.float32), (330, 161003, torch.bfloat16), (170, 160001, torch.float16),
+                                       (260, 190001, torch.float32), (160, 380003, torch.bfloat16),
+                                       (100, 40001, torch.bfloat16), (140, 17001, torch.float32), (60, 70001, torch.float16)])
+def test_policy_rows_shared_by_blocks(obj, n, k, dtype):
+    """Long rows: two or four blocks to a row and more rows than clusters, or no more rows than SMs.  Rows left out,
+    masked whole, with the lowest value throughout or with NaN lie between plain ones; compared with the plain
+    operators, and in place."""
+    coef, t = 0.05, 1.25
+    x = make_logits(k, n, k, dtype, scale=2.0).clone()
+    y = make_labels(k, n, k)
+    y[5::7] = -1
+    empty, lowest, nan = n // 3, n // 3 + 1, n // 2
+    y[empty], y[lowest], y[nan] = 1, 2, 3
+    x[empty] = -math.inf
+    x[lowest] = LOWEST[dtype]
+    x[nan, k - 1] = math.nan
+    mask = torch.ones(n, dtype=torch.bool, device="cuda")
+    mask[[empty, nan]] = False
+    kept = mask & (y >= 0)
+    w = 1.0 / float(kept.sum())
+    z = x.double() / t
+    m = z.max(1, keepdim=True).values
+    lp = (z - m) - (z - m).exp().sum(1, keepdim=True).log()
+    p = lp.exp()
+    want_logp = lp.gather(1, y.clamp(min=0)[:, None])[:, 0]
+    old = torch.where(kept, want_logp, torch.zeros_like(want_logp)).float() - ratios(3, n)
+    adv = torch.randn(n, device="cuda", generator=gen(4))
+    a = obj.policy_loss_logits(x, y, old, adv, mask=mask, entropy_coef=coef, grad_scale=float(n), temperature=t)
+    assert not a.logp[~kept].any() and not a.grad_logits[~kept].any() and torch.isfinite(a.grad_logits).all()
+    plain = torch.where(kept)[0]
+    plain = plain[plain != lowest]
+    tol = float(row_tol(np.full((1, k), float(z[plain].abs().max()))).max())
+    assert float((a.logp.double() - want_logp)[kept].abs().max()) < tol
+    ent = -(p * torch.where(p > 0, lp, torch.zeros_like(lp))).sum(1)
+    assert abs(float(a.entropy) - float(ent[kept].sum()) * w) < tol * (1 + math.log(k))
+    # the loss's gradient to logp, from the operator on the log-probs that were formed
+    parts = obj.policy_loss(a.logp, old, adv, mask=kept)
+    g, ge = parts.grad_logp.double() * n, -coef * w * n
+    # each of log p, H and g is off by at most `tol` of its size, the scale by a few roundings
+    for i in plain.tolist()[:: max(1, n // 24)] + [lowest]:
+        want = (-g[i] * p[i] - ge * p[i] * (lp[i] + ent[i])) / t
+        want[y[i]] += g[i] / t
+        size = (g[i].abs() * p[i] + abs(ge) * p[i] * (lp[i].abs() + ent[i] + 1)) / t
+        size[y[i]] += g[i].abs() / t
+        err = (a.grad_logits[i].double() - want).abs() - (EPS[dtype] * 1.01 * want.abs() + 4 * tol * size + TINY[dtype])
+        assert float(err.max()) <= 0, (i, float(err.max()))
+    b = obj.policy_loss_logits(x, y, old, adv, mask=mask, entropy_coef=coef, grad_scale=float(n), temperature=t, out=x)
+    assert torch.equal(b.grad_logits, a.grad_logits) and torch.equal(b.loss, a.loss) and torch.equal(b.logp, a.logp)
+
+
+@pytest.mark.parametrize("n,k,dtype", [(1, 33000, torch.bfloat16), (30, 33000, torch.float16), (70, 66000, torch.bfloat16),
+                                       (30, 17000, torch.float32), (20, 12000, torch.float16)])
+def test_few_long_rows(obj, n, k, dtype):
+    test_label_logprobs(obj, n, k, dtype)
+    test_label_logprobs_grad(obj, n, k, dtype)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,k", [(40, 20), (40, 300), (20, 9000)])
 def test_gradients_beside_the_logits_and_unlike_aligned(obj, n, k, dtype):

@@ -1031,7 +1031,7 @@ __device__ __forceinline__ RowRec row_rec(const T *row, int K, long long i, int 
 // ahead, so that the others carry no work that is the same for all.
 //
 // ROW_POLICY takes a row's words twice, for the sums and for the gradient; the
-// second time they come from L2, if the rows under way fit there (ring_team).
+// second time they come from L2, if the rows under way fit there (ONE_ROW).
 // Keeping them on the chip instead, in a cluster's shared memory, took 442 us for
 // 4096 x 131072 bf16 against 390: the blocks of a cluster wait for one another
 // twice a row.
@@ -1505,10 +1505,22 @@ static int go_ring(const RowsArgs &a, int &grid, cudaStream_t st) {
         WGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM));
     return launch_rows(kernel, a.rows, R::NT, CL, R::SMEM, cache, a, grid, st);
 }
-// Bytes of a row from which on ROW_POLICY gives an SM one row at a time: the rows
-// under way, three to an SM, would no longer be in L2 when they are read again
-// (65536 bf16 classes: 205 against 239 us for 4096 rows; 50000: 197 against 164).
-constexpr long long ONE_ROW = 112 << 10;
+// ROW_POLICY reads a row again from L2, if the rows under way fit there.  From
+// ONE_ROW bytes on an SM takes one row at a time instead of three (4096 rows of
+// 65536 bf16 classes 205 against 239 us; of 50000, below it, 197 against 164), from
+// ROW_OF_TWO on two SMs share a row (2500 rows of 80000 f32 classes 269 against
+// 316 us, 2000 of 131072 383 against 477; of 70000, below it, 274 against 264), and
+// from ROW_OF_FOUR on four (1500 rows of 200000 f32 classes 478 against 514; of
+// 170000 435 against 417).
+constexpr long long ONE_ROW = 112 << 10, ROW_OF_TWO = 300 << 10, ROW_OF_FOUR = 720 << 10;
+
+// Words of a row from which on a cluster of eight or four blocks shares it where
+// there are fewer rows than SMs.  One row of log-probs of 131072 bf16 classes: 4.9
+// us with eight blocks, 5.7 with four, 9.4 with one; 32768 classes: 4.6, 4.3, 4.9;
+// 8192 classes, below both: 4.6, 4.2, 3.6, since setting up a cluster costs more
+// than it saves.  A policy step of 70 rows of 131072: 14.6 us with four, 21.9 with
+// one.
+constexpr long long CLUSTER_8 = 8192, CLUSTER_4 = 4096;
 
 // Words of a row up to which four warps share it and five rows an SM: a row's
 // joining and closing then waits beside four others (policy step of 16000 x 8000
@@ -1547,13 +1559,17 @@ static int run_rows(const RowsArgs &a, int &grid, cudaStream_t st) {
         return go_rows<T, OP, ENT, 32, 16, 1>(a, grid, st);
     }
     if (alike && a.K < (1ll << 30)) {
+        const long long sms = sm_count(), bytes = a.K * (long long)sizeof(T);
+        if (words >= CLUSTER_8 && a.rows * 8 <= sms) return go_ring<T, OP, ENT, 8, 8>(a, grid, st);
+        if (words >= CLUSTER_4 && a.rows * (words >= CLUSTER_8 ? 2 : 4) <= sms) return go_ring<T, OP, ENT, 8, 4>(a, grid, st);
         if constexpr (OP == ROW_POLICY) {
-            if (a.rows > 3 * sm_count() && a.K * (long long)sizeof(T) >= ONE_ROW) return go_ring<T, OP, ENT, 16, 1>(a, grid, st);
+            if (a.rows > sms && bytes >= ROW_OF_FOUR) return go_ring<T, OP, ENT, 16, 4>(a, grid, st);
+            if (a.rows > sms && bytes >= ROW_OF_TWO) return go_ring<T, OP, ENT, 16, 2>(a, grid, st);
+            // a row an SM, too, where there are no more: 148 rows of 131072 bf16 21 against 29 us
+            if ((a.rows > 3 * sms && bytes >= ONE_ROW) || (a.rows <= sms && words >= CLUSTER_4))
+                return go_ring<T, OP, ENT, 16, 1>(a, grid, st);
         }
-        if (words <= FOUR_WARPS && a.rows > 3 * sm_count()) return go_ring<T, OP, ENT, 4, 1>(a, grid, st);
-        // few rows: as many blocks to a row as the SMs allow
-        if (a.rows * 8 <= sm_count()) return go_ring<T, OP, ENT, 8, 8>(a, grid, st);
-        if (a.rows * 4 <= sm_count()) return go_ring<T, OP, ENT, 8, 4>(a, grid, st);
+        if (words <= FOUR_WARPS && a.rows > 3 * sms) return go_ring<T, OP, ENT, 4, 1>(a, grid, st);
         return go_ring<T, OP, ENT, 8, 1>(a, grid, st);
     }
     static int cache[64];
