@@ -29,6 +29,9 @@ struct Idx {
 };
 
 // A kernel of one part: after the part before it, and the next may be put in place.
+// A part starts once all of the one before has come this far, when the one before
+// that is done.  So what the caller gave (but for the first part), and what the
+// part before the last has written, can be loaded ahead of this.
 __device__ __forceinline__ void part_begin() {
     pdl_wait();
     pdl_trigger();
@@ -290,7 +293,8 @@ __device__ __forceinline__ void quad_mask(const uint8_t *p, long long t, long lo
 // lane l finds the sum up to the l-th boundary of the chunk: a sequence's part is
 // the difference of two, whatever the number of sequences.  add(q, v, n), by one
 // lane each, takes what the range has of sequence q.  `start` gets the range's
-// first place, for the parts to come.
+// first place, for the parts to come.  What is loaded first is loaded ahead of the
+// wait for the part before.
 template <bool VALUES, int PER>
 struct Tokens {
     unsigned keep;
@@ -298,20 +302,24 @@ struct Tokens {
 };
 template <bool VALUES, int PER, typename FETCH, typename ADD>
 __device__ __forceinline__ void range_by_seq(const Idx &off, long long S, const Range &r, Place *start, FETCH fetch, ADD add) {
-    if (r.a >= r.b) return;
+    if (r.a >= r.b) {
+        part_begin();
+        return;
+    }
     constexpr int CHUNK = 32 * PER;
     constexpr unsigned FULL = 0xffffffffu;
     const int lane = threadIdx.x & 31;
     Tokens<VALUES, PER> more = fetch(r.a + lane * PER);
     Place at;
     at.find(off, S, 0, r.a);
-    if (lane == 0) start[warp_index()] = at;
     long long q = at.q;                // sequence that the warp is in, -1 and S as in Place
     double sum = 0.0;                  // of it, by lane
     int count = 0;
     long long b = LLONG_MAX;           // lane l: the end of sequence q + l
     auto ends = [&]() { b = q + 1 + lane <= S ? off.at(q + 1 + lane) : LLONG_MAX; };
     ends();
+    part_begin();
+    if (lane == 0) start[warp_index()] = at;
     auto give = [&](long long to, double v, int n) {
         if (n && to >= 0 && to < S) add(to, v, n);
     };
@@ -480,8 +488,9 @@ constexpr int PAIR_EACH = 4;  // pairs of a thread under way together: they are 
 // Bytes: 13 a token read and 4 written, 16 a pair and the gathers of its
 // scores.  With many pairs time goes to the gathers and to the atomics of their
 // gradients: two a pair, which a bound on their terms allows for (the square loss
-// has none and takes up to four).  2000000 pairs of 1000000 rows: 54 to 61 us
-// (HBM alone 8), of which the pairs' part takes 40 with L2 at 0.62 of its
+// has none and takes up to four).  2000000 pairs of 1000000 rows: 56 us
+// (HBM alone 8; 61 with the indices loaded after the wait), of which the pairs' part
+// takes 40 with L2 at 0.62 of its
 // throughput.  4096 pairs of 3.3 million tokens: 32 us (HBM alone 6.5), the start of
 // each of the four parts' chains of loads.
 // The bound on a pair's gradient, from the blocks' largest weights.
@@ -552,12 +561,9 @@ __device__ __forceinline__ void pref_pairs(const PrefArgs &a, double *scratch) {
     using S = Score<RAGGED>;
     const long long me = (long long)blockIdx.x * NT + threadIdx.x, all = (long long)gridDim.x * NT;
     const bool bounded = a.rule.kind != 2;
-    const GridSums grid_sums = pref_grid_sums(a);
-    double total = 0.0;
-    for (long long p0 = me; p0 < a.P; p0 += all * PAIR_EACH) {
-        long long c[PAIR_EACH], r[PAIR_EACH];
-        S dc[PAIR_EACH], dr[PAIR_EACH];
-        float wt[PAIR_EACH];
+    long long c[PAIR_EACH], r[PAIR_EACH];
+    float wt[PAIR_EACH];
+    auto fetch = [&](long long p0) {
 #pragma unroll
         for (int e = 0; e < PAIR_EACH; ++e) {
             const long long p = p0 + e * all;
@@ -565,6 +571,14 @@ __device__ __forceinline__ void pref_pairs(const PrefArgs &a, double *scratch) {
             r[e] = p < a.P ? a.rejected.at(p) : -1;
             wt[e] = a.weight && p < a.P ? a.weight[p] : 1.0f;
         }
+    };
+    fetch(me);
+    part_begin();
+    const GridSums grid_sums = pref_grid_sums(a);
+    double total = 0.0;
+    for (long long p0 = me; p0 < a.P; p0 += all * PAIR_EACH) {
+        S dc[PAIR_EACH], dr[PAIR_EACH];
+        if (p0 != me) fetch(p0);
 #pragma unroll
         for (int e = 0; e < PAIR_EACH; ++e) {
             dc[e] = seq_score<RAGGED>(a, c[e]);
@@ -624,6 +638,15 @@ __device__ __forceinline__ void pref_row_grad(const PrefArgs &a, double *scratch
 template <int NT>
 __device__ __forceinline__ void pref_grad(const PrefArgs &a, double *scratch) {
     const bool bounded = a.rule.kind != 2;
+    const Range range = a.cut.range();
+    const int lane = threadIdx.x & 31;
+    Place at{-1, 0, 0};
+    bool more[4] = {};
+    if (range.a < range.b) {  // the places are the part before the last's
+        at = a.places[warp_index()];
+        quad_mask(a.mask, range.a + lane * 4, a.T, a.whole_mask, more);
+    }
+    part_begin();
     const GridSums grid_sums = pref_grid_sums(a);
     const double inv = a.P ? 1.0 / (double)a.P : 0.0;
     pref_loss<NT>(a, inv, scratch);
@@ -631,10 +654,7 @@ __device__ __forceinline__ void pref_grad(const PrefArgs &a, double *scratch) {
         const double v = (bounded ? grid_sums.value(q) : a.grads.value(q)) * inv;
         return (float)(a.rule.average && a.count[q] ? v / (double)a.count[q] : v);
     };
-    const Range range = a.cut.range();
-    const int lane = threadIdx.x & 31;
     if (range.a >= range.b) return;
-    Place at = a.places[warp_index()];
     float of = 0.0f, held = 0.0f;  // of the sequence that the warp is in, and of the next, loaded ahead
     long long held_q = -2;
     auto enter = [&]() {
@@ -643,8 +663,6 @@ __device__ __forceinline__ void pref_grad(const PrefArgs &a, double *scratch) {
         held = held_q >= 0 && held_q < a.S ? grad_of(held_q) : 0.0f;
     };
     enter();
-    bool more[4];
-    quad_mask(a.mask, range.a + lane * 4, a.T, a.whole_mask, more);
     for (long long t0 = range.a; t0 < range.b; t0 += STEP) {
         const long long t1 = t0 + STEP < range.b ? t0 + STEP : range.b, t = t0 + lane * 4;
         bool keep[4];
@@ -682,7 +700,7 @@ __device__ __forceinline__ void pref_grad(const PrefArgs &a, double *scratch) {
 template <int PART>
 __global__ void __launch_bounds__(GRID_THREADS) k_pref_part(const __grid_constant__ PrefArgs a) {
     __shared__ double scratch[33];
-    part_begin();
+    if (PART == 0 || PART == 5) part_begin();  // the others have loads that can go ahead
     if (PART == 0) pref_start<GRID_THREADS>(a);
     if (PART == 1) pref_sums(a);
     if (PART == 2) pref_pairs<true, GRID_THREADS>(a, scratch);
@@ -854,6 +872,7 @@ __device__ __forceinline__ void policy_count(const CountArgs &a, double *scratch
             }
         }
     } else {
+        part_begin();
         for (long long t = r.a + (threadIdx.x & 31) * 4; t < r.b; t += STEP) {
             bool keep[4];
             quad_mask(a.mask, t, a.T, a.whole_mask, keep);
@@ -874,7 +893,6 @@ __global__ void __launch_bounds__(GRID_THREADS) k_policy_zero(const __grid_const
 }
 __global__ void __launch_bounds__(GRID_THREADS) k_policy_count(const __grid_constant__ CountArgs a) {
     __shared__ double scratch[33];
-    part_begin();
     policy_count(a, scratch);
 }
 __global__ void __launch_bounds__(BLOCK_THREADS) k_policy_count_block(const __grid_constant__ CountArgs a) {
@@ -911,13 +929,12 @@ struct PolicyTokens {
     bool whole;
 };
 // Bytes: 17 a token read (and its mask byte twice), 4 written.  4 million tokens by
-// 4001 sequences: 38 to 46 us (HBM alone 10), half of it counting; issue and chains
-// of loads bound both.
+// 4001 sequences: 36.5 us (HBM alone 10; 46 with nothing loaded ahead of the wait for
+// the part before), a third of it counting; issue and chains of loads bound both.
 __device__ __forceinline__ void policy_tokens(const PolicyTokens &a, double *scratch) {
     const CountArgs &n = a.count;
     double sum[POL_STATS] = {};
     const PolicyRule &rule = a.rule;
-    const float w_all = rule.by_sequence ? 0.0f : token_weight(n.cnt);
     const Range r = n.cut.range();
     const int lane = threadIdx.x & 31;
     // a step's values are loaded while the step before is worked on
@@ -935,6 +952,8 @@ __device__ __forceinline__ void policy_tokens(const PolicyTokens &a, double *scr
 #pragma unroll
     for (int j = 0; j < 4; ++j) more.adv[j] = more.ref[j] = 0.0f;
     if (r.a < r.b) fetch(r.a + lane * 4);
+    part_begin();
+    const float w_all = rule.by_sequence ? 0.0f : token_weight(n.cnt);
     Place at{0, LLONG_MAX, LLONG_MAX};
     float wt = w_all, av = 0.0f;  // of the sequence that the warp is in
     bool in = true;
@@ -1033,7 +1052,6 @@ __device__ __forceinline__ void policy_tokens(const PolicyTokens &a, double *scr
 }
 __global__ void __launch_bounds__(GRID_THREADS, 3) k_policy_tokens(const __grid_constant__ PolicyTokens a) {
     __shared__ double scratch[33];
-    part_begin();
     policy_tokens(a, scratch);
 }
 __global__ void __launch_bounds__(BLOCK_THREADS) k_policy_tokens_block(const __grid_constant__ PolicyTokens a) {
