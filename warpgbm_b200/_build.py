@@ -15,14 +15,14 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libwgb_b200.so")
-SOURCES = ["wgb_lib.cu", "wgb_engine.cu", "wgb_ops.cu", "wgb_io.cu", "wgb_quantile.cu", "wgb_noalloc.cu", "wgb_comm.cu", "wgb_decode.cu", "wgb_objectives.cu", "wgb_logits.cu", "wgb_common.cuh"]
+UNITS = ["wgb_lib.cu", "wgb_objectives_lib.cu"]  # compiled at the same time, each the same from build to build
+SOURCES = [*UNITS, "wgb_engine.cu", "wgb_ops.cu", "wgb_io.cu", "wgb_quantile.cu", "wgb_noalloc.cu", "wgb_comm.cu", "wgb_decode.cu", "wgb_objectives.cu", "wgb_logits.cu", "wgb_common.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-pthread", "-shared",
     "-Xptxas", "-warn-spills",
-    "--split-compile=0",  # as many threads as there are cores: the kernels come in many types
 ]
 
 
@@ -46,7 +46,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not needs_build():
         return LIB
     tmp = LIB + ".tmp"
-    cmd = [_nvcc(), *NVCC_FLAGS, "-o", tmp, os.path.join(CSRC, "wgb_lib.cu"), "-lpthread", "-ldl"]
+    cmd = [_nvcc(), *NVCC_FLAGS, "--threads", str(len(UNITS)), "-o", tmp, *(os.path.join(CSRC, u) for u in UNITS),
+           "-lpthread", "-ldl"]
     if verbose:
         print(" ".join(cmd))
     r = subprocess.run(cmd, capture_output=True, text=True)

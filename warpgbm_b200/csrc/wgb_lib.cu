@@ -1,5 +1,6 @@
-// Single translation unit of libwgb_b200.so: the level-wise engine and the
-// binning / prediction / reference-compatible entry points share kernels.
+// Translation unit of libwgb_b200.so for all but the objectives
+// (wgb_objectives_lib.cu): the level-wise engine and the binning / prediction /
+// reference-compatible entry points share kernels.
 #include "wgb_engine.cu"
 #include "wgb_ops.cu"
 #include "wgb_io.cu"
@@ -7,5 +8,3 @@
 #include "wgb_noalloc.cu"
 #include "wgb_comm.cu"
 #include "wgb_decode.cu"
-#include "wgb_objectives.cu"
-#include "wgb_logits.cu"

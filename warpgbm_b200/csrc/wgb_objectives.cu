@@ -287,6 +287,18 @@ __device__ __forceinline__ void quad_mask(const uint8_t *p, long long t, long lo
     }
 }
 
+// The same as a word, a byte that is not zero for each token that is kept, and such
+// a word's bits.
+__device__ __forceinline__ unsigned quad_mask_word(const uint8_t *p, long long t, long long T, bool whole) {
+    if (p && whole && t + 4 <= T) return *reinterpret_cast<const unsigned *>(p + t);
+    bool k[4];
+    quad_mask(p, t, T, whole, k);
+    return (unsigned)k[0] | (unsigned)k[1] << 8 | (unsigned)k[2] << 16 | (unsigned)k[3] << 24;
+}
+__device__ __forceinline__ unsigned quad_mask_bits(unsigned w) {
+    return ((__vcmpne4(w, 0u) & 0x08040201u) * 0x01010101u) >> 24 & 15u;
+}
+
 // Sums of a warp's range by sequence.  A lane has PER neighbouring tokens of a
 // chunk of 32 PER: fetch(t) gives the tokens from t on, as `keep` bits and, with
 // VALUES, `v`.  The chunk's sums up to each lane's first token are scanned, and
@@ -488,10 +500,9 @@ constexpr int PAIR_EACH = 4;  // pairs of a thread under way together: they are 
 // Bytes: 13 a token read and 4 written, 16 a pair and the gathers of its
 // scores.  With many pairs time goes to the gathers and to the atomics of their
 // gradients: two a pair, which a bound on their terms allows for (the square loss
-// has none and takes up to four).  2000000 pairs of 1000000 rows: 56 us
-// (HBM alone 8; 61 with the indices loaded after the wait), of which the pairs' part
-// takes 40 with L2 at 0.62 of its
-// throughput.  4096 pairs of 3.3 million tokens: 32 us (HBM alone 6.5), the start of
+// has none and takes up to four).  2000000 pairs of 1000000 rows: 57 us
+// (HBM alone 8), of which the pairs' part takes 40 with L2 at 0.62 of its
+// throughput.  4096 pairs of 3.3 million tokens: 29.4 us (HBM alone 6.5), the start of
 // each of the four parts' chains of loads.
 // The bound on a pair's gradient, from the blocks' largest weights.
 __device__ __forceinline__ GridSums pref_grid_sums(const PrefArgs &a) {
@@ -635,16 +646,24 @@ __device__ __forceinline__ void pref_row_grad(const PrefArgs &a, double *scratch
     }
 }
 // The gradient of every token: its sequence's, where it is kept.
-template <int NT>
+// AHEAD: steps whose masks are loaded together.  One alone leaves a warp waiting
+// (4096 pairs 30.2 against 29.4 us with four); a block of 1024 threads has no
+// registers for more (8 pairs 12.8 against 14.1).
+template <int NT, int AHEAD>
 __device__ __forceinline__ void pref_grad(const PrefArgs &a, double *scratch) {
     const bool bounded = a.rule.kind != 2;
     const Range range = a.cut.range();
     const int lane = threadIdx.x & 31;
     Place at{-1, 0, 0};
-    bool more[4] = {};
+    unsigned more[AHEAD] = {};
+    auto fetch = [&](long long t0) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (t0 + i * STEP < range.b) more[i] = quad_mask_word(a.mask, t0 + i * STEP + lane * 4, a.T, a.whole_mask);
+    };
     if (range.a < range.b) {  // the places are the part before the last's
         at = a.places[warp_index()];
-        quad_mask(a.mask, range.a + lane * 4, a.T, a.whole_mask, more);
+        fetch(range.a);
     }
     part_begin();
     const GridSums grid_sums = pref_grid_sums(a);
@@ -663,13 +682,18 @@ __device__ __forceinline__ void pref_grad(const PrefArgs &a, double *scratch) {
         held = held_q >= 0 && held_q < a.S ? grad_of(held_q) : 0.0f;
     };
     enter();
-    for (long long t0 = range.a; t0 < range.b; t0 += STEP) {
+    unsigned kept = 0;  // four bits a step
+    int left = 0;       // steps that it has
+    for (long long t0 = range.a; t0 < range.b; t0 += STEP, kept >>= 4, --left) {
         const long long t1 = t0 + STEP < range.b ? t0 + STEP : range.b, t = t0 + lane * 4;
-        bool keep[4];
         float g[4];
+        if (!left) {
+            left = AHEAD;
+            kept = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) keep[j] = more[j];
-        if (t1 < range.b) quad_mask(a.mask, t + STEP, a.T, a.whole_mask, more);
+            for (int i = 0; i < AHEAD; ++i) kept |= quad_mask_bits(more[i]) << (4 * i);
+            fetch(t0 + AHEAD * STEP);
+        }
         if (many_seqs(a.off, a.S, at, t1)) {
             const long long first = at.q;
             at.find(a.off, a.S, at.q + 1, t1 - 1);
@@ -692,7 +716,7 @@ __device__ __forceinline__ void pref_grad(const PrefArgs &a, double *scratch) {
             }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) g[j] = keep[j] ? g[j] : 0.0f;
+        for (int j = 0; j < 4; ++j) g[j] = kept >> j & 1u ? g[j] : 0.0f;
         quad_store(a.grad, t, a.T, a.whole, g);
     }
 }
@@ -705,7 +729,7 @@ __global__ void __launch_bounds__(GRID_THREADS) k_pref_part(const __grid_constan
     if (PART == 1) pref_sums(a);
     if (PART == 2) pref_pairs<true, GRID_THREADS>(a, scratch);
     if (PART == 4) pref_pairs<false, GRID_THREADS>(a, scratch);
-    if (PART == 3) pref_grad<GRID_THREADS>(a, scratch);
+    if (PART == 3) pref_grad<GRID_THREADS, 4>(a, scratch);
     if (PART == 5) pref_row_grad<GRID_THREADS>(a, scratch);
 }
 __global__ void __launch_bounds__(BLOCK_THREADS) k_pref_block(const __grid_constant__ PrefArgs a) {
@@ -720,7 +744,7 @@ __global__ void __launch_bounds__(BLOCK_THREADS) k_pref_block(const __grid_const
     if (a.off.p) pref_pairs<true, BLOCK_THREADS>(a, scratch);
     else pref_pairs<false, BLOCK_THREADS>(a, scratch);
     __syncthreads();
-    if (a.off.p) pref_grad<BLOCK_THREADS>(a, scratch);
+    if (a.off.p) pref_grad<BLOCK_THREADS, 1>(a, scratch);
     else pref_row_grad<BLOCK_THREADS>(a, scratch);
 }
 
@@ -844,8 +868,7 @@ __device__ __forceinline__ void policy_count(const CountArgs &a, double *scratch
                     const uint4 m = *reinterpret_cast<const uint4 *>(a.mask + t);
                     const unsigned w[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)  // a bit for each byte that is not zero
-                        x.keep |= (((__vcmpne4(w[i], 0u) & 0x08040201u) * 0x01010101u) >> 24 & 15u) << (4 * i);
+                    for (int i = 0; i < 4; ++i) x.keep |= quad_mask_bits(w[i]) << (4 * i);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
@@ -929,7 +952,7 @@ struct PolicyTokens {
     bool whole;
 };
 // Bytes: 17 a token read (and its mask byte twice), 4 written.  4 million tokens by
-// 4001 sequences: 36.5 us (HBM alone 10; 46 with nothing loaded ahead of the wait for
+// 4001 sequences: 36.5 us (HBM alone 10; 38.8 with nothing loaded ahead of the wait for
 // the part before), a third of it counting; issue and chains of loads bound both.
 __device__ __forceinline__ void policy_tokens(const PolicyTokens &a, double *scratch) {
     const CountArgs &n = a.count;
