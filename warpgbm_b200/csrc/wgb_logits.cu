@@ -1037,9 +1037,9 @@ __device__ __forceinline__ RowRec row_rec(const T *row, int K, long long i, int 
 // twice a row.
 //
 // Measured at 4096 x 131072 bf16 (1.07 GB): log-probs 161 us, HBM at its copy
-// rate; policy step 388 us, 0.84 of it, the exponential unit busy for 0.63 of the
-// time (two a logit).  Their gradient alone at 2047 x 50001 f16: 0.9 of the copy
-// rate.
+// rate; policy step 387 us (420 on a slower machine), 0.84 of it, the exponential
+// unit busy for 0.63 of the time (two a logit).  Their gradient alone at 2047 x
+// 50001 f16: 0.9 of the copy rate.
 //
 // In place a gradient is written only after the whole row is read: the row's own
 // words, its ends and the label's logit all go into what a warp puts.
